@@ -48,6 +48,15 @@ typedef struct ssmi_index ssmi_index;
  * and every search path returns the fp32 result up to summation order.  Other fp32 values are rounded to nearest
  * even at add (8 significant bits: coarser than SSMI_F16's 11). */
 #define SSMI_BF16 2
+/* 8-bit rows (Flat indexes): e4m3 codes (OCP: largest finite value 448, 0x7f / 0xff = NaN, no infinity) with one power-of-two
+ * scale for every 128 of them, value = code * 2^(b - 127) for the scale byte b (255 = NaN).  A row of d elements is
+ * SSMI_F8_LD(d) codes - whole blocks, zero codes behind d - and SSMI_F8_BLOCKS(d) scale bytes.  Quantising takes the smallest power of
+ * two s with max|x| <= 448 s over the block (not below 2^-127) and rounds x / s to nearest even: a quarter of the bytes of
+ * fp32, every element off by at most 2^-4 of itself (or 2^-10 s, where that is more), and quantising what a row stands for
+ * gives a row of the same values.  A block with an infinity or a NaN in it becomes NaN. */
+#define SSMI_F8 3
+#define SSMI_F8_LD(d) (((d) + 127) / 128 * 128)
+#define SSMI_F8_BLOCKS(d) (((d) + 127) / 128)
 /* where a caller buffer lives */
 #define SSMI_HOST 0
 #define SSMI_DEVICE 1
@@ -187,6 +196,45 @@ int ssmi_index_write(ssmi_index* h, const char* path);
 int ssmi_index_write_append(ssmi_index* h, const char* path);
 /* replaces faiss.read_index(path)                  core/index_manager.py:185 */
 int ssmi_index_read(const char* path, int storage_dtype, int device, ssmi_index** out);
+
+/* ---- 8-bit rows --------------------------------------------------------- */
+/* What feeds an index of SSMI_F8 storage, and the product it is built on (no reference counterpart: its embedder ends in a
+ * root-mean-square norm and F.normalize, core/qwen3_vl_embedding.py:447-448, and hands fp32 rows to FAISS).  All pointers are
+ * DEVICE memory of `device`; work is enqueued on `stream` (NULL = the HIP null stream), nothing is allocated or waited for,
+ * so the calls may be captured into a graph.  Code rows: 16-byte aligned, codes_stride a multiple of 16 bytes >= SSMI_F8_LD(d);
+ * scale rows: 4-byte aligned and readable to a multiple of 4 bytes, scales_stride a multiple of 4 bytes >= SSMI_F8_BLOCKS(d).  Strides of plain rows are in
+ * elements.  Outputs must not overlap inputs, unless stated. */
+/* (n, d) rows of src_dtype (SSMI_F32 / F16 / BF16) -> 8-bit rows; the codes behind d are written as zeros */
+int ssmi_f8_quantize(int device, int64_t n, int d, const void* x, int src_dtype, int64_t x_stride, uint8_t* codes,
+                     int64_t codes_stride, uint8_t* scales, int64_t scales_stride, void* stream);
+/* 8-bit rows -> (n, d) rows of out_dtype */
+int ssmi_f8_dequantize(int device, int64_t n, int d, const uint8_t* codes, int64_t codes_stride, const uint8_t* scales,
+                       int64_t scales_stride, void* out, int out_dtype, int64_t out_stride, void* stream);
+/* The norm that ends in 8-bit rows.  h = x + residual, rounded to dtype and stored in residual_out (which may be residual or x
+ * itself); without a residual (NULL) h = x.  y = h / sqrt(mean(h^2) + eps) * weight (NULL: 1), sums in fp32; unit != 0:
+ * y / max(|y|_2, 1e-12), what goes into an inner-product index.  codes / scales receive y.  d <= 32768. */
+int ssmi_f8_rms_norm(int device, int64_t n, int d, const void* x, int dtype, int64_t x_stride, const void* residual,
+                     int64_t residual_stride, void* residual_out, int64_t residual_out_stride, const void* weight,
+                     int weight_dtype, float eps, int unit, uint8_t* codes, int64_t codes_stride, uint8_t* scales,
+                     int64_t scales_stride, void* stream);
+/* out (m, n) of out_dtype (SSMI_F16 or SSMI_BF16): inner products of the m rows of a with the n rows of b, k elements each.
+ * fp32 accumulators on the matrix cores; the instruction aligns the products of a block to the largest and drops what is more
+ * than 13 bits below it, which a 16-bit output does not show and an fp32 one would. */
+int ssmi_f8_matmul(int device, int64_t m, int64_t n, int k, const uint8_t* a_codes, int64_t a_stride, const uint8_t* a_scales,
+                   int64_t a_scales_stride, const uint8_t* b_codes, int64_t b_stride, const uint8_t* b_scales,
+                   int64_t b_scales_stride, void* out, int out_dtype, int64_t out_stride, void* stream);
+/* ssmi_index_add of rows that are 8-bit already (an index of SSMI_F8 storage; device memory of its GPU): kept bit for bit.
+ * The caller's writes to them must have completed. */
+int ssmi_index_add_f8(ssmi_index* h, int64_t n, const uint8_t* codes, int64_t codes_stride, const uint8_t* scales,
+                      int64_t scales_stride);
+/* ssmi_index_search_min of queries that are 8-bit already (device buffers throughout; returns after enqueueing).  An index of
+ * SSMI_F8 storage quantises fp32 queries by ssmi_f8_quantize, so both calls give the same results.  Scores are the inner
+ * products of the 8-bit query with the 8-bit rows summed in 64 bits and rounded once to fp32, so a query gets the same answer
+ * in any batch; candidates are chosen by the matrix cores' sums (off by about 1e-6 |q||x|) with 16 spare ones, so a row can
+ * only be missed where more than 16 rows lie within that error of the k-th score.  NaN scores are never reported.
+ * k <= 1008 (the other searches of such an index too). */
+int ssmi_index_search_f8(ssmi_index* h, int64_t nq, const uint8_t* codes, int64_t codes_stride, const uint8_t* scales,
+                         int64_t scales_stride, int k, float min_score, float* D, int64_t* I, int64_t id_offset, void* stream);
 
 /* ---- introspection ------------------------------------------------------ */
 typedef struct ssmi_timing {

@@ -16,6 +16,7 @@ from .faiss_compat import (  # noqa: F401
     read_index,
     write_index,
 )
+from .f8 import F8Rows, matmul_f8, quantize_f8, rms_norm_f8  # noqa: F401
 from .index_factory import (  # noqa: F401
     INDEX_TYPE_DESCRIPTIONS,
     IndexConfig,
@@ -25,5 +26,5 @@ from .index_factory import (  # noqa: F401
 
 __all__ = [
     "faiss_compat", "IndexFlatIP", "IndexIVFFlat", "METRIC_INNER_PRODUCT", "METRIC_L2", "read_index",
-    "write_index", "INDEX_TYPE_DESCRIPTIONS", "IndexConfig", "IndexFactory", "IndexType",
+    "write_index", "F8Rows", "quantize_f8", "rms_norm_f8", "matmul_f8", "INDEX_TYPE_DESCRIPTIONS", "IndexConfig", "IndexFactory", "IndexType",
 ]

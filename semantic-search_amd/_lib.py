@@ -17,7 +17,7 @@ import torch  # noqa: F401  (must precede the CDLL below, see module docstring)
 _HERE = Path(__file__).resolve().parent
 LIB_PATH = _HERE / "csrc" / "libssmi.so"
 
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, F8 = 0, 1, 2, 3
 HOST, DEVICE = 0, 1
 KIND_FLAT, KIND_IVFFLAT = 0, 1
 MAX_K = 1024
@@ -36,6 +36,9 @@ class Timing(ctypes.Structure):
         ("last_grid", ctypes.c_int),
     ]
 
+
+# 8-bit rows: codes, their stride, scales, their stride
+_F8_ROWS = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64]
 
 # name -> (argtypes); every function returns int except ssmi_last_error
 _SIGNATURES = {
@@ -79,6 +82,16 @@ _SIGNATURES = {
     "ssmi_index_write": [_c_index_p, ctypes.c_char_p],
     "ssmi_index_write_append": [_c_index_p, ctypes.c_char_p],
     "ssmi_index_read": [ctypes.c_char_p, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_c_index_p)],
+    "ssmi_f8_quantize": [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, *_F8_ROWS, ctypes.c_void_p],
+    "ssmi_f8_dequantize": [ctypes.c_int, ctypes.c_int64, ctypes.c_int, *_F8_ROWS, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p],
+    "ssmi_f8_rms_norm": [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p,
+                         ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int,
+                         *_F8_ROWS, ctypes.c_void_p],
+    "ssmi_f8_matmul": [ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, *_F8_ROWS, *_F8_ROWS, ctypes.c_void_p, ctypes.c_int,
+                       ctypes.c_int64, ctypes.c_void_p],
+    "ssmi_index_add_f8": [_c_index_p, ctypes.c_int64, *_F8_ROWS],
+    "ssmi_index_search_f8": [_c_index_p, ctypes.c_int64, *_F8_ROWS, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p,
+                             ctypes.c_int64, ctypes.c_void_p],
     "ssmi_index_get_timing": [_c_index_p, ctypes.POINTER(Timing)],
     "ssmi_index_get_scan_times": [_c_index_p, ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int)],
     "ssmi_index_set_shadow_policy": [_c_index_p, ctypes.c_int],

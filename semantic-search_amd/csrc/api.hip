@@ -3,6 +3,7 @@
 #include "../../include/ssmi.h"
 #include "kernels.h"
 #include "index.h"
+#include "f8.h"
 
 #include <cstdarg>
 #include <cstdio>
@@ -37,7 +38,7 @@ int RowStore::init(int d_, int dtype_, hipStream_t stream) {
     d = d_;
     dtype = dtype_;
     elsize = (size_t)dtype_elsize(dtype);
-    ld = (d + 7) / 8 * 8;
+    ld = dtype == SSMI_F8 ? f8_ld(d) : (d + 7) / 8 * 8;
     row_bytes = (size_t)ld * elsize;
     // ~1 GiB segments, between 2^10 and 2^24 rows
     seg_shift = 10;
@@ -50,6 +51,18 @@ int RowStore::init(int d_, int dtype_, hipStream_t stream) {
     if (env) { int v = atoi(env); if (v >= 8 && v <= 24) seg_shift = v; }
     nrows = 0;
     seg0_cap = 0;
+    HIPCHECK(hipMalloc((void**)&d_segs, sizeof(void*) * kMaxSegs));
+    HIPCHECK(zero_device_sync(d_segs, sizeof(void*) * kMaxSegs, stream));
+    return 0;
+}
+
+int RowStore::init_scales(const RowStore& codes, hipStream_t stream) {
+    d = f8_blocks(codes.d);
+    dtype = codes.dtype;
+    elsize = 1;
+    ld = (d + 15) / 16 * 16;
+    row_bytes = (size_t)ld;
+    seg_shift = codes.seg_shift;
     HIPCHECK(hipMalloc((void**)&d_segs, sizeof(void*) * kMaxSegs));
     HIPCHECK(zero_device_sync(d_segs, sizeof(void*) * kMaxSegs, stream));
     return 0;
@@ -159,7 +172,7 @@ static int create_common(int d, int storage_dtype, int device, int kind, ssmi_in
     if (!out) return fail("out is NULL");
     *out = nullptr;
     if (d < 1 || d > 65536) return fail("dimension %d out of range [1, 65536]", d);
-    if (!dtype_known(storage_dtype)) return fail("unknown storage dtype %d", storage_dtype);
+    if (!storage_known(storage_dtype)) return fail("unknown storage dtype %d", storage_dtype);
     int ndev = 0;
     HIPCHECK(hipGetDeviceCount(&ndev));
     if (device < 0 || device >= ndev) return fail("device %d not available (%d visible)", device, ndev);
@@ -192,6 +205,7 @@ static int create_common(int d, int storage_dtype, int device, int kind, ssmi_in
     if (const char* e = getenv("SSMI_SHADOW_DTYPE")) h->shadow_pref = !strcmp(e, "f16") ? SSMI_F16 : (!strcmp(e, "bf16") ? SSMI_BF16 : -1);
     HIPCHECK(hipMalloc((void**)&h->d_flag, 256));
     CHECK(h->rows.init(d, storage_dtype, h->stream));
+    if (storage_dtype == SSMI_F8) CHECK(h->scales.init_scales(h->rows, h->stream));
     guard.h = nullptr;
     *out = h;
     return 0;
@@ -250,6 +264,7 @@ int ssmi_index_free(ssmi_index* h) {
     if (h->ev_order) (void)hipEventDestroy(h->ev_order);
     ivf_destroy(h);
     h->rows.destroy();
+    h->scales.destroy();
     if (h->has_shadow) h->shadow16.destroy();
     for (int i = 0; i < kWsSlots; ++i) if (h->ws[i]) (void)hipFree(h->ws[i]);
     if (h->tail_counters) (void)hipFree(h->tail_counters);
@@ -307,6 +322,7 @@ int ssmi_index_set_nprobe(ssmi_index* h, int nprobe) {
 namespace ssmi {
 // Append n rows (host or device, fp32 or fp16) to a row store, converting/padding as needed.
 int store_add(ssmi_index* h, RowStore& R, int64_t n, const void* x, int src_dtype, int mem_kind) {
+    if (R.dtype == SSMI_F8) return f8_store_add(h, n, x, src_dtype, mem_kind);
     const long long row0 = R.nrows;
     if ((unsigned long long)(row0 + n) >= 0xFFFFFFFFull) return fail("index would exceed 2^32-2 vectors");
     CHECK(R.reserve(row0 + n, h->stream));
@@ -372,6 +388,7 @@ int ssmi_index_add_random_unit(ssmi_index* h, int64_t n, uint64_t seed) {
     DeviceGuard g(h->device);
     quiesce(h);
     if (h->kind != SSMI_KIND_FLAT) return ivf_add_random_unit(h, n, seed);
+    if (h->rows.dtype == SSMI_F8) return f8_add_random_unit(h, n, seed);
     RowStore& R = h->rows;
     const long long row0 = R.nrows;
     if ((unsigned long long)(row0 + n) >= 0xFFFFFFFFull) return fail("index would exceed 2^32-2 vectors");
@@ -574,7 +591,9 @@ int ssmi_index_search_min(ssmi_index* h, int64_t nq, const float* q, int q_mem_k
     if (nq == 0) return 0;
     if (!q || !D || !I) return fail("NULL buffer");
     if (k < 1) return fail("k must be >= 1");
-    if (k > kMaxK) return fail("k=%d exceeds the supported maximum %d", k, kMaxK);
+    const bool f8 = h->rows.dtype == SSMI_F8;
+    const int max_k = f8 ? kF8MaxK : kMaxK;  // 8-bit rows: 16 spare candidates are scored again in 64 bits
+    if (k > max_k) return fail("k=%d exceeds the supported maximum %d", k, max_k);
     if (nq > (1ll << 24)) return fail("nq too large");
     if (min_score != min_score) return fail("min_score is NaN");
     // f32_to_ord(min_score); -FLT_MAX or below (incl. -inf) = no floor, encoded as 0
@@ -624,7 +643,11 @@ int ssmi_index_search_min(ssmi_index* h, int64_t nq, const float* q, int q_mem_k
         HIPCHECK(launch_fill_empty(Ddev, Idev, nq * k, s));
     } else {
         const float* qdev = nullptr;
-        if (pin) {
+        int64_t q_stride = h->rows.ld;
+        if (f8 && q_mem_kind == SSMI_DEVICE) {
+            qdev = q;  // the conversion to 8-bit rows pads by itself
+            q_stride = h->rows.d;
+        } else if (pin) {
             const RowStore& R = h->rows;
             float* qpin = (float*)pin;
             if (R.ld == R.d) {
@@ -641,7 +664,8 @@ int ssmi_index_search_min(ssmi_index* h, int64_t nq, const float* q, int q_mem_k
         } else {
             CHECK(stage_queries(h, nq, q, q_mem_kind, s, &qdev));
         }
-        if (h->kind == SSMI_KIND_FLAT) CHECK(store_search(h, h->rows, nq, qdev, k, Ddev, Idev, id_offset, s, true, nullptr, min_ord));
+        if (f8) CHECK(f8_store_search(h, nq, F8Queries{qdev, q_stride, nullptr, 0, nullptr, 0}, k, Ddev, Idev, id_offset, s, min_ord));
+        else if (h->kind == SSMI_KIND_FLAT) CHECK(store_search(h, h->rows, nq, qdev, k, Ddev, Idev, id_offset, s, true, nullptr, min_ord));
         else CHECK(ivf_search(h, nq, qdev, k, Ddev, Idev, id_offset, s, min_ord));
     }
     if (pin) {  // (D, I) sit back to back in workspace 3: one copy, then out of the pinned block
@@ -713,7 +737,7 @@ int gather_by_ids(ssmi_index* h, int64_t n, const int64_t* ids, float* out, bool
         HIPCHECK(hipMemsetAsync(bad, 0, 4, h->stream));
         RowView v = R.view();
         if (h->kind == SSMI_KIND_IVFFLAT) v.nrows = h->ivf_slots_used;
-        HIPCHECK(launch_gather_rows(v, R.dtype, dids, cnt, R.d, dout, bad, h->stream));
+        HIPCHECK(gather_store_rows(h, R, v.nrows, dids, cnt, dout, bad, h->stream));
         if (!out_on_device)
             HIPCHECK(hipMemcpyAsync(out + (size_t)done * R.d, dout, (size_t)cnt * R.d * 4, hipMemcpyDeviceToHost, h->stream));
         HIPCHECK(hipStreamSynchronize(h->stream));
@@ -772,7 +796,8 @@ int ssmi_index_score_ids(ssmi_index* h, int64_t n, const int64_t* ids, int n_neg
     HIPCHECK(hipMemsetAsync(bad, 0, 4, h->stream));
     RowView v = R.view();
     if (h->kind == SSMI_KIND_IVFFLAT) v.nrows = h->ivf_slots_used;
-    HIPCHECK(launch_score_rows(v, R.dtype, dids, n, R.d, dneg, n_neg, dout, bad, h->stream));
+    if (R.dtype == SSMI_F8) HIPCHECK(launch_f8_score_rows(F8View{v, (const void* const*)h->scales.d_segs, h->scales.ld}, dids, n, R.d, dneg, n_neg, dout, bad, h->stream));
+    else HIPCHECK(launch_score_rows(v, R.dtype, dids, n, R.d, dneg, n_neg, dout, bad, h->stream));
     HIPCHECK(hipMemcpyAsync(out_host, dout, (size_t)n * n_neg * 4, hipMemcpyDeviceToHost, h->stream));
     HIPCHECK(hipStreamSynchronize(h->stream));
     return 0;

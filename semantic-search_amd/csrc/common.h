@@ -37,10 +37,12 @@ __host__ __device__ inline uint32_t key_id(skey_t k) { return 0xFFFFFFFFu - (uin
 
 #define SSMI_NEG_MAX (-3.402823466e+38f)
 
-// element types of the row stores (include/ssmi.h: SSMI_F32 / SSMI_F16 / SSMI_BF16)
-__host__ __device__ inline int dtype_elsize(int dtype) { return dtype == 0 ? 4 : 2; }
+// element types of the row stores (include/ssmi.h: SSMI_F32 / SSMI_F16 / SSMI_BF16 / SSMI_F8)
+__host__ __device__ inline int dtype_elsize(int dtype) { return dtype == 0 ? 4 : dtype == 3 ? 1 : 2; }
 __host__ __device__ inline bool dtype_is16(int dtype) { return dtype == 1 || dtype == 2; }
+// types a caller's rows may have (8-bit rows come with scales: f8.h)
 __host__ __device__ inline bool dtype_known(int dtype) { return dtype >= 0 && dtype <= 2; }
+__host__ __device__ inline bool storage_known(int dtype) { return dtype >= 0 && dtype <= 3; }
 
 // bfloat16 storage element: the upper half of an fp32.  Widening is a shift (exact), narrowing rounds to nearest
 // even (NaN stays NaN); no arithmetic is ever done in this type.

@@ -1,0 +1,97 @@
+// f8.h - 8-bit rows: e4m3 codes with one power-of-two scale for every 128 of them (internal to libssmi).
+//
+//   value(row, e) = code(row, e) * 2^(b(row, e / 128) - 127)
+//
+// codes: OCP e4m3 (largest finite value 448, no infinity, 0x7f / 0xff = NaN), rows padded with zero codes to whole blocks.
+// b: E8M0 exponent bytes, 255 = NaN.  The quantiser takes the smallest power of two s with max|x| <= 448 s and rounds x / s
+// to nearest even.  Powers of two, for two reasons: v_mfma_scale_f32_16x16x128_f8f6f4 takes one E8M0 byte per operand row and
+// block of K = 128 and applies it for nothing, and quantising the values of a quantised row gives the same values (a block
+// whose largest code rounded down to 224 halves its scale and doubles its codes).
+#pragma once
+#include "kernels.h"
+
+namespace ssmi {
+
+static constexpr int kF8 = 3;             // SSMI_F8
+static constexpr int kF8Block = 128;      // codes per scale
+static constexpr int kF8Spare = 16;       // candidates beyond k that a search scores again in 64 bits
+static constexpr int kF8MaxNorm = 32768;  // elements of a row that the norm keeps in registers
+static constexpr int kF8MaxK = kMaxK - kF8Spare;
+
+inline int f8_ld(int d) { return (d + kF8Block - 1) / kF8Block * kF8Block; }
+inline int f8_blocks(int d) { return (d + kF8Block - 1) / kF8Block; }
+
+// n rows of codes and scales in plain memory; strides in bytes
+struct F8Mat {
+    const unsigned char* codes;
+    long long stride;         // multiple of 16, codes 16-byte aligned
+    const unsigned char* scales;
+    long long sstride;        // multiple of 4, scales 4-byte aligned
+    long long n;
+};
+// the same inside a row store: segment tables of the codes (X) and of the scales
+struct F8View {
+    RowView X;                // ld = codes per row
+    const void* const* ssegs;
+    int sld;                  // scale bytes per row (multiple of 16)
+};
+
+struct F8NormArgs {
+    const void* x; long long x_stride;                 // strides in elements
+    const void* residual; long long r_stride;          // nullptr: none
+    void* residual_out; long long ro_stride;
+    const void* weight; int weight_dtype;              // nullptr: none
+    float eps;
+    bool norm, unit;
+    long long n;
+    int d, dtype;
+    unsigned char* codes; long long stride;
+    unsigned char* scales; long long sstride;
+};
+hipError_t launch_f8_rows(const F8NormArgs& a, int num_cu, hipStream_t s);
+// codes + scales -> (n, d) of out_dtype, row stride in elements
+hipError_t launch_f8_dequantize(const F8Mat& m, int d, void* out, int out_dtype, long long out_stride, int num_cu, hipStream_t s);
+// rows by id out of a row store -> fp32 (n, d); as launch_gather_rows / launch_score_rows
+hipError_t launch_f8_gather(const F8View& v, const int64_t* ids, long long n, int d, float* out, int* bad, hipStream_t s);
+hipError_t launch_f8_score_rows(const F8View& v, const int64_t* ids, long long n, int d, const float* neg, int n_neg, float* out,
+                                int* bad, hipStream_t s);
+// out[i][j] = <a_i, b_j>, (a.n, b.n) of out_dtype (SSMI_F16 / SSMI_BF16), row stride in elements
+hipError_t launch_f8_matmul(const F8Mat& a, const F8Mat& b, int k, void* out, int out_dtype, long long out_stride, int num_cu, hipStream_t s);
+
+// search over a row store: the k best of every query with their scores summed in 64 bits
+struct F8SearchPlan {
+    int kp;                   // candidates kept per query by the first pass: min(k + kF8Spare, kMaxK)
+    int parts;                // partial lists per query
+    bool scan;                // streaming scan (few queries), else the tile kernel
+    int bt, r, threads, grid_x, grid_y;
+    int tq, nqt, nslices, gtop_m;
+    long long rows_per_slice;
+    size_t lds, partial_bytes, cand_bytes, share_bytes;
+    const char* kernel;
+};
+bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8SearchPlan* p);
+hipError_t launch_f8_search(const F8View& v, const F8Mat& q, int k, const F8SearchPlan& p, void* share, void* cand, skey_t* partial,
+                            const TailMerge& tail, hipStream_t s);
+// ids (q.n, kp) of the first pass (-1: none) -> (D, I) (q.n, k)
+hipError_t launch_f8_finish(const F8View& v, const F8Mat& q, const int64_t* ids, int kp, int k, float* D, int64_t* I,
+                            int64_t id_offset, unsigned min_ord, hipStream_t s);
+
+#ifdef __HIPCC__
+// two e4m3 codes per call from the low or high half of a word
+template <bool HI>
+__device__ __forceinline__ void f8_unpack2(unsigned w, float& a, float& b) {
+    const auto v = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, HI);
+    a = v[0];
+    b = v[1];
+}
+__device__ __forceinline__ void f8_unpack4(unsigned w, float (&o)[4]) {
+    f8_unpack2<false>(w, o[0], o[1]);
+    f8_unpack2<true>(w, o[2], o[3]);
+}
+// 2^(b - 127); 255: NaN.  (2^-127 is a subnormal fp32.)
+__device__ __forceinline__ float f8_scale(unsigned b) {
+    return b == 255u ? __builtin_nanf("") : __uint_as_float(b ? b << 23 : 0x00400000u);
+}
+#endif
+
+}  // namespace ssmi

@@ -26,6 +26,7 @@ struct RowStore {
     void** d_segs = nullptr;
 
     int init(int d, int dtype, hipStream_t stream);  // `stream`: where the segment table is zeroed (see zero_device_sync)
+    int init_scales(const RowStore& codes, hipStream_t stream);  // 8-bit rows: the scale bytes of `codes`, segment by segment
     void destroy();
     int reserve(long long total_rows, hipStream_t stream);
     RowView view() const;
@@ -38,6 +39,7 @@ struct ssmi_index {
     int device = 0;
     int num_cu = 256;
     ssmi::RowStore rows;  // Flat: the database.  IVF: the slot store (pages of list members)
+    ssmi::RowStore scales;  // SSMI_F8: one scale byte per 128 codes of `rows` (f8.h); rows and segments as there
     // fp16 copy of an fp32 Flat database, built lazily by the first large-batch search so that
     // it can run on the MFMA kernel (costs +50 % HBM; batch-1..8 searches keep using the fp32 rows)
     ssmi::RowStore shadow16;
@@ -157,6 +159,23 @@ struct ProbePlanRequest {
 };
 int store_search(ssmi_index* h, const RowStore& R, int64_t nq, const float* qdev, int k, float* Ddev, int64_t* Idev,
                  int64_t id_offset, hipStream_t s, bool record, ProbePlanRequest* plan = nullptr, unsigned min_ord = 0);
+
+// f8_api.hip: the same for 8-bit rows.  Queries: fp32 rows of q_stride elements, or 8-bit rows as they are
+struct F8Queries {
+    const float* f32;
+    int64_t q_stride;
+    const unsigned char* codes;
+    int64_t stride;
+    const unsigned char* scales;
+    int64_t sstride;
+};
+int f8_store_add(ssmi_index* h, int64_t n, const void* x, int src_dtype, int mem_kind);
+int f8_add_random_unit(ssmi_index* h, int64_t n, uint64_t seed);
+int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float* Ddev, int64_t* Idev, int64_t id_offset, hipStream_t s,
+                    unsigned min_ord);
+// rows by id -> fp32, whatever the row type (launch_gather_rows and its 8-bit form)
+hipError_t gather_store_rows(ssmi_index* h, const RowStore& R, long long view_rows, const int64_t* ids, long long n, float* out, int* bad,
+                             hipStream_t s);
 
 // static_search.hip: resolves this device's copy of the static scratch array (once per device, device current)
 int static_scratch_setup(int device);

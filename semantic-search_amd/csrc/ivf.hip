@@ -1279,6 +1279,7 @@ int ssmi_index_create_ivfflat(int d, int nlist, int storage_dtype, int device, s
     if (!out) return fail("out is NULL");
     *out = nullptr;
     if (nlist < 1) return fail("nlist must be >= 1");
+    if (storage_dtype == SSMI_F8) return fail("8-bit rows: Flat indexes only");
     ssmi_index* h = nullptr;
     CHECK(ssmi_index_create_flat(d, storage_dtype, device, &h));
     h->kind = SSMI_KIND_IVFFLAT;

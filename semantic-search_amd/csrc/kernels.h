@@ -69,6 +69,8 @@ hipError_t launch_score_rows(const RowView& X, int dtype, const int64_t* ids, lo
 // K10: append unit-norm gaussian rows [row0,row0+n)
 hipError_t launch_fill_random_unit(const RowView& X, int dtype, void* const* segs_rw, long long row0, long long n,
                                    int d, uint64_t seed, hipStream_t s);
+// the same rows as a plain fp32 (n, d) array
+hipError_t launch_random_unit(float* out, long long row0, long long n, int d, uint64_t seed, hipStream_t s);
 // fp32 store rows -> 16-bit shadow store rows (dst_dtype 1 = fp16, 2 = bf16); *inexact (device int, may be null) is
 // set when some value does not survive the narrowing exactly
 hipError_t launch_shadow_rows(const RowView& src, void* const* dsegs, int dshift, int dst_dtype, long long row0, long long n,

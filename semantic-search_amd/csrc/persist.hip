@@ -63,9 +63,7 @@ int read_rows(ssmi_index* h, const RowStore& R, long long view_rows, const int64
         float* dout = (float*)((char*)h->ws[0] + ids_bytes + 256);
         HIPCHECK(hipMemcpyAsync(dids, slots + done, (size_t)cnt * 8, hipMemcpyHostToDevice, h->stream));
         HIPCHECK(hipMemsetAsync(bad, 0, 4, h->stream));
-        RowView v = R.view();
-        v.nrows = view_rows;
-        HIPCHECK(launch_gather_rows(v, R.dtype, dids, cnt, R.d, dout, bad, h->stream));
+        HIPCHECK(gather_store_rows(h, R, view_rows, dids, cnt, dout, bad, h->stream));
         HIPCHECK(hipMemcpyAsync(out + (size_t)done * R.d, dout, (size_t)cnt * R.d * 4, hipMemcpyDeviceToHost, h->stream));
         HIPCHECK(hipStreamSynchronize(h->stream));
     }

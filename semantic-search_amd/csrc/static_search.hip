@@ -67,6 +67,7 @@ int ssmi_index_search_static(ssmi_index* h, int64_t nq, const float* q_dev, int 
     if (nq == 0) return 0;
     if (!q_dev || !D_dev || !I_dev) return fail("NULL buffer");
     if (k < 1) return fail("k must be >= 1");
+    if (h->rows.dtype == SSMI_F8) return fail("search_static: not for 8-bit rows (their search needs workspaces of the handle)");
     if (k > kMaxK) return fail("k=%d exceeds the supported maximum %d", k, kMaxK);
     const RowStore& R = h->rows;
     if (R.ld != R.d)

@@ -145,7 +145,7 @@ __device__ __forceinline__ void normal4(long long row, int quad, uint64_t seed, 
 // one wave per row; two passes (norm, then regenerate + scale + store)
 template <typename T>
 __global__ void fill_random_unit_kernel(void* const* segs, int seg_shift, int ld, long long row0, long long n, int d,
-                                        uint64_t seed) {
+                                        uint64_t seed, float* flat) {
     const int lane = lane_id();
     const long long i = (long long)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
     if (i >= n) return;
@@ -160,7 +160,8 @@ __global__ void fill_random_unit_kernel(void* const* segs, int seg_shift, int ld
     }
     ss = wave_sum(ss);
     const float inv = rsqrtf(ss > 1e-30f ? ss : 1e-30f);
-    T* dst = reinterpret_cast<T*>(row_ptr_rw(segs, seg_shift, row, (size_t)ld * sizeof(T)));
+    // flat: the rows go to a plain (n, ld) array instead of a row store
+    T* dst = flat ? reinterpret_cast<T*>(flat) + (size_t)i * ld : reinterpret_cast<T*>(row_ptr_rw(segs, seg_shift, row, (size_t)ld * sizeof(T)));
     for (int qd = lane; qd < nquad; qd += 64) {
         float z[4];
         normal4(row, qd, seed, z);
@@ -177,9 +178,15 @@ hipError_t launch_fill_random_unit(const RowView& X, int dtype, void* const* seg
     if (n <= 0) return hipSuccess;
     const int wpb = 4;
     const dim3 grid((unsigned)((n + wpb - 1) / wpb)), block(64 * wpb);
-    if (dtype == 0) hipLaunchKernelGGL((fill_random_unit_kernel<float>), grid, block, 0, s, segs_rw, X.seg_shift, X.ld, row0, n, d, seed);
-    else if (dtype == 1) hipLaunchKernelGGL((fill_random_unit_kernel<__half>), grid, block, 0, s, segs_rw, X.seg_shift, X.ld, row0, n, d, seed);
-    else hipLaunchKernelGGL((fill_random_unit_kernel<bf16_t>), grid, block, 0, s, segs_rw, X.seg_shift, X.ld, row0, n, d, seed);
+    if (dtype == 0) hipLaunchKernelGGL((fill_random_unit_kernel<float>), grid, block, 0, s, segs_rw, X.seg_shift, X.ld, row0, n, d, seed, (float*)nullptr);
+    else if (dtype == 1) hipLaunchKernelGGL((fill_random_unit_kernel<__half>), grid, block, 0, s, segs_rw, X.seg_shift, X.ld, row0, n, d, seed, (float*)nullptr);
+    else hipLaunchKernelGGL((fill_random_unit_kernel<bf16_t>), grid, block, 0, s, segs_rw, X.seg_shift, X.ld, row0, n, d, seed, (float*)nullptr);
+    return hipGetLastError();
+}
+
+hipError_t launch_random_unit(float* out, long long row0, long long n, int d, uint64_t seed, hipStream_t s) {
+    if (n <= 0) return hipSuccess;
+    hipLaunchKernelGGL((fill_random_unit_kernel<float>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, (void* const*)nullptr, 0, d, row0, n, d, seed, out);
     return hipGetLastError();
 }
 

@@ -1,0 +1,187 @@
+"""8-bit rows: quantisation, the norm that ends in them, and their product (libssmi.so, csrc/f8_*.hip).
+
+A row is e4m3 codes with one power-of-two scale for every 128 of them, kept as its biased exponent:
+value = code * 2**(scale - 127).  `IndexFlatIP(d, storage="f8")` keeps such rows: `add` and `search` quantise what they are given,
+or take an `F8Rows` as it is - for instance what `rms_norm_f8(..., unit=True)` makes of a model's last hidden states, which is
+what the reference's embedder does in fp32 before it hands rows to FAISS (core/qwen3_vl_embedding.py:447-448).
+
+All calls work on tensors of a ROCm device, enqueue on its current torch stream, wait for nothing and may be captured into a
+graph.  Argument errors raise ValueError or TypeError, errors of the engine RuntimeError.
+"""
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+BLOCK = 128
+_SRC = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def _blocks(d: int) -> int:
+    return (d + BLOCK - 1) // BLOCK
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _rows_arg(x, what: str) -> torch.Tensor:
+    """A 2-D device tensor of a known type whose rows are contiguous (other layouts are copied)."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what}: expected a torch tensor, got {type(x).__name__}")
+    if not x.is_cuda:
+        raise ValueError(f"{what}: the tensor must live on a ROCm device")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"{what}: expected a 2-D tensor with at least one column, got shape {tuple(x.shape)}")
+    if x.dtype not in _SRC:
+        raise TypeError(f"{what}: expected float32, float16 or bfloat16, got {x.dtype}")
+    return x if x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+
+
+def _stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+class F8Rows:
+    """n rows of d elements in 8 bits: `codes` (n, whole blocks of 128) float8_e4m3fn, `scales` (n, >= blocks) uint8."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, d: int):
+        self.codes, self.scales, self.d = codes, scales, int(d)
+
+    @classmethod
+    def empty(cls, n: int, d: int, device) -> "F8Rows":
+        """Rows to be written by quantize_f8 / rms_norm_f8 (`out=`)."""
+        blocks = _blocks(d)
+        return cls(torch.empty((n, blocks * BLOCK), dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty((n, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=device), d)
+
+    @classmethod
+    def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, d: Optional[int] = None) -> "F8Rows":
+        """Rows from codes (n, d or whole blocks; float8_e4m3fn or uint8) and scale exponents (n, blocks; uint8).  The tensors
+        are used as they are where their layout allows; codes behind d are set to zero."""
+        if codes.dim() != 2 or scales.dim() != 2 or codes.shape[0] != scales.shape[0]:
+            raise ValueError(f"F8Rows: expected 2-D codes and scales of as many rows, got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        if not codes.is_cuda or codes.device != scales.device:
+            raise ValueError("F8Rows: codes and scales must live on the same ROCm device")
+        if codes.dtype not in (torch.float8_e4m3fn, torch.uint8) or scales.dtype != torch.uint8:
+            raise TypeError(f"F8Rows: expected float8_e4m3fn or uint8 codes and uint8 scales, got {codes.dtype} and {scales.dtype}")
+        d = int(codes.shape[1] if d is None else d)
+        blocks = _blocks(d)
+        if d < 1 or codes.shape[1] not in (d, blocks * BLOCK) or scales.shape[1] < blocks:
+            raise ValueError(f"F8Rows: {d} elements need {d} or {blocks * BLOCK} codes and {blocks} scales a row, got {codes.shape[1]} and {scales.shape[1]}")
+        raw = codes.view(torch.uint8)
+        if raw.shape[1] != blocks * BLOCK or raw.stride(1) != 1 or raw.stride(0) % 16 or raw.data_ptr() % 16 or raw.stride(0) < blocks * BLOCK:
+            fresh = torch.zeros((raw.shape[0], blocks * BLOCK), dtype=torch.uint8, device=raw.device)
+            fresh[:, :d] = raw[:, :d]
+            raw = fresh
+        elif d < blocks * BLOCK:
+            raw[:, d:].zero_()
+        if scales.stride(1) != 1 or scales.stride(0) % 4 or scales.data_ptr() % 4 or min(scales.shape[1], scales.stride(0)) < (blocks + 3) // 4 * 4:
+            fresh = torch.zeros((scales.shape[0], (blocks + 3) // 4 * 4), dtype=torch.uint8, device=scales.device)
+            fresh[:, :blocks] = scales[:, :blocks]
+            scales = fresh
+        return cls(raw.view(torch.float8_e4m3fn), scales, d)
+
+    @property
+    def n(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def __len__(self) -> int:
+        return self.n
+
+    def __getitem__(self, rows: slice) -> "F8Rows":
+        """A contiguous range of the rows (a view)."""
+        if not isinstance(rows, slice) or rows.step not in (None, 1):
+            raise TypeError("F8Rows: only plain slices of rows")
+        return F8Rows(self.codes[rows], self.scales[rows], self.d)
+
+    def _abi(self):
+        """(codes, stride, scales, stride) as the C entry points take them."""
+        c, s = self.codes, self.scales
+        return (c.data_ptr(), c.stride(0) if self.n > 1 else c.shape[1], s.data_ptr(), s.stride(0) if self.n > 1 else (s.shape[1] + 3) // 4 * 4)
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values the rows stand for, (n, d); exact in float32 and bfloat16 (four significant bits times a power of two)."""
+        if dtype not in _SRC:
+            raise TypeError(f"dequantize: expected float32, float16 or bfloat16, got {dtype}")
+        out = torch.empty((self.n, self.d), dtype=dtype, device=self.device)
+        _lib.check(_lib.load().ssmi_f8_dequantize(self.device.index, self.n, self.d, *self._abi(), out.data_ptr(), _SRC[dtype], self.d, _stream(self.device)))
+        return out
+
+
+def _out_rows(out: Optional[F8Rows], n: int, d: int, device: torch.device, what: str) -> F8Rows:
+    if out is None:
+        return F8Rows.empty(n, d, device)
+    if not isinstance(out, F8Rows) or out.n != n or out.d != d or out.device != device:
+        raise ValueError(f"{what}: out must be F8Rows of {n} rows of {d} elements on {device}")
+    return out
+
+
+def quantize_f8(x: torch.Tensor, out: Optional[F8Rows] = None) -> F8Rows:
+    """8-bit rows of x (n, d): per 128 elements the smallest power of two s with max|x| <= 448 s, codes x / s to nearest even."""
+    x = _rows_arg(x, "quantize_f8")
+    n, d = x.shape
+    out = _out_rows(out, n, d, x.device, "quantize_f8")
+    _lib.check(_lib.load().ssmi_f8_quantize(x.device.index, n, d, x.data_ptr(), _SRC[x.dtype], _stride(x), *out._abi(), _stream(x.device)))
+    return out
+
+
+def rms_norm_f8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                residual_out: Optional[torch.Tensor] = None, eps: float = 1e-6, unit: bool = False, out: Optional[F8Rows] = None) -> F8Rows:
+    """8-bit rows of the root-mean-square norm of h = x + residual: h / sqrt(mean(h^2) + eps) * weight, sums in float32.
+
+    The sum is rounded to x's type and stored in `residual_out` (default: back into `residual`).  unit=True: rows of unit length,
+    ready for an inner-product index."""
+    x = _rows_arg(x, "rms_norm_f8")
+    n, d = x.shape
+    w = r = ro = None
+    if weight is not None:
+        if not isinstance(weight, torch.Tensor) or weight.shape != (d,) or weight.device != x.device:
+            raise ValueError(f"rms_norm_f8: weight must be a tensor of {d} elements on {x.device}")
+        if weight.dtype not in _SRC:
+            raise TypeError(f"rms_norm_f8: weight must be float32, float16 or bfloat16, got {weight.dtype}")
+        w = weight.contiguous()
+    if residual is not None:
+        r = residual
+        ro = residual if residual_out is None else residual_out
+        for t, name in ((r, "residual"), (ro, "residual_out")):
+            if not isinstance(t, torch.Tensor) or t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+                raise ValueError(f"rms_norm_f8: {name} must be like x: shape {tuple(x.shape)}, {x.dtype}, {x.device}")
+        if d > 1 and ro.stride(1) != 1 or n > 1 and ro.stride(0) < d:
+            raise ValueError("rms_norm_f8: residual_out must have contiguous rows")
+        if d > 1 and r.stride(1) != 1 or n > 1 and r.stride(0) < d:
+            r = r.contiguous()
+    elif residual_out is not None:
+        raise ValueError("rms_norm_f8: residual_out without a residual")
+    out = _out_rows(out, n, d, x.device, "rms_norm_f8")
+    _lib.check(_lib.load().ssmi_f8_rms_norm(
+        x.device.index, n, d, x.data_ptr(), _SRC[x.dtype], _stride(x), r.data_ptr() if r is not None else None, _stride(r) if r is not None else 0,
+        ro.data_ptr() if ro is not None else None, _stride(ro) if ro is not None else 0, w.data_ptr() if w is not None else None,
+        _SRC[w.dtype] if w is not None else 0, float(eps), 1 if unit else 0, *out._abi(), _stream(x.device)))
+    return out
+
+
+def matmul_f8(a: F8Rows, b: F8Rows, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """(a.n, b.n): inner products of the rows of a (activations) with the rows of b (weights, or a table of embeddings)."""
+    if not isinstance(a, F8Rows) or not isinstance(b, F8Rows):
+        raise TypeError("matmul_f8: expected two F8Rows")
+    if a.d != b.d:
+        raise ValueError(f"matmul_f8: rows of {a.d} and {b.d} elements")
+    if a.device != b.device:
+        raise ValueError(f"matmul_f8: operands on {a.device} and {b.device}")
+    if out is not None:
+        out_dtype = out.dtype
+    if out_dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"matmul_f8: the output is float16 or bfloat16, not {out_dtype}")
+    if out is None:
+        out = torch.empty((a.n, b.n), dtype=out_dtype, device=a.device)
+    elif out.shape != (a.n, b.n) or out.device != a.device or (b.n > 1 and out.stride(1) != 1) or (a.n > 1 and out.stride(0) < b.n):
+        raise ValueError(f"matmul_f8: out must be ({a.n}, {b.n}) with contiguous rows on {a.device}")
+    _lib.check(_lib.load().ssmi_f8_matmul(a.device.index, a.n, b.n, a.d, *a._abi(), *b._abi(), out.data_ptr(), _SRC[out_dtype],
+                                          out.stride(0) if a.n > 1 else b.n, _stream(a.device)))
+    return out

@@ -18,7 +18,8 @@ Flat objects deliberately have no `nlist` / `nprobe` / `hnsw` attributes, becaus
 get_index_stats / set_search_params branch on hasattr (core/index_factory.py:230-236,317-320).
 
 Additive (not in the reference): `storage="f16"` / `storage="bf16"` row storage (bf16 is LOSSLESS for the
-reference's embeddings, which are bf16 model outputs cast to fp32: core/model_wrapper.py:201-203), torch tensors on a
+reference's embeddings, which are bf16 model outputs cast to fp32: core/model_wrapper.py:201-203), `storage="f8"` for Flat
+indexes (8-bit rows with block scales, f8.py: a quarter of the bytes of fp32, `add` / `search` also take `F8Rows`), torch tensors on a
 ROCm device accepted by add/search (device pointers are handed straight to the
 kernels), `search(..., id_offset=)` for row-sharded databases, `reconstruct_batch`.
 
@@ -33,14 +34,15 @@ import numpy as np
 import torch
 
 from . import _lib
+from .f8 import F8Rows
 
 _NO_FLOOR = -3.4028234663852886e38  # -FLT_MAX: ssmi_index_search_min's "no score floor"
 METRIC_INNER_PRODUCT = 0
 METRIC_L2 = 1
 
 _STORAGE = {"f32": _lib.F32, "fp32": _lib.F32, "float32": _lib.F32, "f16": _lib.F16, "fp16": _lib.F16,
-            "float16": _lib.F16, "bf16": _lib.BF16, "bfloat16": _lib.BF16}
-_STORAGE_NAME = {_lib.F32: "f32", _lib.F16: "f16", _lib.BF16: "bf16"}
+            "float16": _lib.F16, "bf16": _lib.BF16, "bfloat16": _lib.BF16, "f8": _lib.F8, "fp8": _lib.F8, "float8": _lib.F8}
+_STORAGE_NAME = {_lib.F32: "f32", _lib.F16: "f16", _lib.BF16: "bf16", _lib.F8: "f8"}
 # torch dtypes the engine takes as they are (anything else is widened to float32 first)
 _TORCH_SRC = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
@@ -162,8 +164,28 @@ class _IndexBase:
         if x.device.index != self.device:
             raise RuntimeError(f"{what}: tensor is on {x.device}, index lives on cuda:{self.device}")
 
+    def _check_f8(self, x: F8Rows, what: str) -> None:
+        assert x.d == self.d, f"{what}: dimension {x.d} != index dimension {self.d}"
+        if x.device.index != self.device:
+            raise RuntimeError(f"{what}: rows are on {x.device}, index lives on cuda:{self.device}")
+
+    def _device_out(self, out, nq: int, k: int, device):
+        """Result tensors of a device search: the caller's (views of one gather buffer, say) or new ones."""
+        if out is not None:
+            D, I = out
+            if (tuple(D.shape) != (nq, k) or tuple(I.shape) != (nq, k) or D.dtype != torch.float32 or
+                    I.dtype != torch.int64 or not D.is_contiguous() or not I.is_contiguous() or D.device != device):
+                raise ValueError("search: out must be contiguous (nq,k) float32 / int64 tensors on the index's device")
+            return D, I
+        return torch.empty((nq, k), dtype=torch.float32, device=device), torch.empty((nq, k), dtype=torch.int64, device=device)
+
     def add(self, x) -> None:
         """Append vectors; ids are the running row numbers (FAISS add() without ids)."""
+        if isinstance(x, F8Rows):
+            self._check_f8(x, "add")
+            torch.cuda.current_stream(x.device).synchronize()  # the library copies on its own stream
+            _lib.check(self._lib.ssmi_index_add_f8(self._handle(), x.n, *x._abi()))
+            return
         if isinstance(x, torch.Tensor) and x.is_cuda:
             self._check_tensor(x, "add")
             x, dt = _device_rows(x)
@@ -194,20 +216,20 @@ class _IndexBase:
         if k < 1:
             raise RuntimeError("search: k must be >= 1")
         floor = _floor32(min_score)
+        if isinstance(x, F8Rows):  # device tensors out, enqueued on the current torch stream
+            self._check_f8(x, "search")
+            D, I = self._device_out(out, x.n, k, x.device)
+            stream = torch.cuda.current_stream(x.device).cuda_stream
+            _lib.check(self._lib.ssmi_index_search_f8(self._handle(), x.n, *x._abi(), k, floor, D.data_ptr(), I.data_ptr(),
+                                                      int(id_offset), stream))
+            return D, I
         if isinstance(x, torch.Tensor) and x.is_cuda:
             if x.dim() == 1:
                 x = x.reshape(1, -1)
             self._check_tensor(x, "search")
             x = x.contiguous().float()
             nq = x.shape[0]
-            if out is not None:  # caller-provided contiguous (nq,k) device tensors (e.g. views of one gather buffer)
-                D, I = out
-                if (tuple(D.shape) != (nq, k) or tuple(I.shape) != (nq, k) or D.dtype != torch.float32 or
-                        I.dtype != torch.int64 or not D.is_contiguous() or not I.is_contiguous() or D.device != x.device):
-                    raise ValueError("search: out must be contiguous (nq,k) float32 / int64 tensors on the index's device")
-            else:
-                D = torch.empty((nq, k), dtype=torch.float32, device=x.device)
-                I = torch.empty((nq, k), dtype=torch.int64, device=x.device)
+            D, I = self._device_out(out, nq, k, x.device)
             stream = torch.cuda.current_stream(x.device).cuda_stream
             _lib.check(self._lib.ssmi_index_search_min(self._handle(), nq, x.data_ptr(), _lib.DEVICE, k, floor, D.data_ptr(),
                                                        I.data_ptr(), _lib.DEVICE, int(id_offset), stream))
