@@ -9,6 +9,9 @@
 // whose largest code rounded down to 224 halves its scale and doubles its codes).
 #pragma once
 #include "kernels.h"
+#ifdef __HIPCC__
+#include "topk.h"
+#endif
 
 namespace ssmi {
 
@@ -63,18 +66,35 @@ struct F8SearchPlan {
     int kp;                   // candidates kept per query by the first pass: min(k + kF8Spare, kMaxK)
     int parts;                // partial lists per query
     bool scan;                // streaming scan (few queries), else the tile kernel
-    int bt, r, threads, grid_x, grid_y;
-    int tq, nqt, nslices, gtop_m;
+    int bt, r, threads, grid_x;
+    int nb;                   // scan: blocks per row where that is 1, 2 or 4, 8 where it is a multiple of 8, else 0
+    int cap, every;           // scan: candidates a query's buffer holds, turns of three stages between two looks at them
+    int tq, nqt, nslices;
     long long rows_per_slice;
     size_t lds, partial_bytes, cand_bytes, share_bytes;
     const char* kernel;
 };
 bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8SearchPlan* p);
-hipError_t launch_f8_search(const F8View& v, const F8Mat& q, int k, const F8SearchPlan& p, void* share, void* cand, skey_t* partial,
-                            const TailMerge& tail, hipStream_t s);
-// ids (q.n, kp) of the first pass (-1: none) -> (D, I) (q.n, k)
-hipError_t launch_f8_finish(const F8View& v, const F8Mat& q, const int64_t* ids, int kp, int k, float* D, int64_t* I,
-                            int64_t id_offset, unsigned min_ord, hipStream_t s);
+hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& p, void* share, void* cand, skey_t* partial, hipStream_t s);
+// the streaming scan of up to p.bt queries, and what follows the first pass; queries: fp32 rows of d elements at f32, else q.codes
+struct F8ScanArgs {
+    F8View v;
+    F8Mat q;
+    const float* f32;
+    long long f32_stride;     // elements
+    bool f32_vec;             // rows of 16-byte aligned floats
+    int d, k, kp;
+    skey_t* partial;          // [q.n][p.parts][kp]
+    unsigned* counter;        // ticket counter, zero between launches: the scan does everything (one query); nullptr: launch_f8_finish follows
+    unsigned* shared;         // eight words, zero between searches: the highest threshold of every query (f32_to_ord bits); nullptr: none
+    float* D;
+    int64_t* I;
+    int64_t id_offset;
+    unsigned min_ord;
+    int cap, every;
+};
+hipError_t launch_f8_scan(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s);
+hipError_t launch_f8_finish(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s);
 
 #ifdef __HIPCC__
 // two e4m3 codes per call from the low or high half of a word
@@ -87,6 +107,34 @@ __device__ __forceinline__ void f8_unpack2(unsigned w, float& a, float& b) {
 __device__ __forceinline__ void f8_unpack4(unsigned w, float (&o)[4]) {
     f8_unpack2<false>(w, o[0], o[1]);
     f8_unpack2<true>(w, o[2], o[3]);
+}
+// Eight neighbouring elements of a block whose other elements the 16 lanes of this lane's row hold -> their codes and the
+// block's scale byte.  e0: place of the first in a row of d elements.  All 16 lanes call.
+__device__ __forceinline__ uint2 f8_pack8(const float (&v)[8], int e0, int d, unsigned& b) {
+    // largest magnitude of the block as an integer: NaN > infinity > every finite value
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+    m = max(m, (unsigned)xor_lane<1>((int)m));
+    m = max(m, (unsigned)xor_lane<2>((int)m));
+    m = max(m, (unsigned)xor_lane<4>((int)m));
+    m = max(m, (unsigned)xor_lane<8>((int)m));
+    if (m < 0x7f800000u) {
+        // m = f * 2^(E-127), 1 <= f < 2, and 448 = 1.75 * 2^8
+        b = (unsigned)max((int)(m >> 23) - 8 + ((m & 0x7fffffu) > 0x600000u ? 1 : 0), 0);
+        const float inv = __uint_as_float((254u - b) << 23);
+        int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, lo, true);
+        int hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, 0, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, hi, true);
+        return uint2{(unsigned)lo, (unsigned)hi};
+    }
+    // an infinity or a NaN makes its block NaN; the padding keeps its zero codes
+    b = 255u;
+    unsigned w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j >> 2] |= e0 + j < d ? 0x7fu << (8 * (j & 3)) : 0u;
+    return uint2{w[0], w[1]};
 }
 // 2^(b - 127); 255: NaN.  (2^-127 is a subnormal fp32.)
 __device__ __forceinline__ float f8_scale(unsigned b) {

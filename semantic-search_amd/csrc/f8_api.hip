@@ -4,6 +4,7 @@
 #include "f8.h"
 #include "index.h"
 #include <algorithm>
+#include <atomic>
 
 using namespace ssmi;
 
@@ -35,7 +36,11 @@ int check_plain(const char* what, const void* p, int dtype, int64_t stride, int6
     return 0;
 }
 int num_cu_of(int device, int* out) {
+    static std::atomic<int> known[64];   // asked once per device
+    *out = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+    if (*out) return 0;
     HIPCHECK(hipDeviceGetAttribute(out, hipDeviceAttributeMultiprocessorCount, device));
+    if (device < 64) known[device].store(*out, std::memory_order_relaxed);
     return 0;
 }
 
@@ -129,7 +134,7 @@ hipError_t gather_store_rows(ssmi_index* h, const RowStore& R, long long view_ro
     return launch_gather_rows(v, R.dtype, ids, n, R.d, out, bad, s);
 }
 
-// Workspaces: 4 query codes and scales, 5 candidate buffers, 2 partial lists, 6 first-pass (D, I), 7 shared thresholds.
+// Workspaces: 4 query codes and scales, 5 candidate buffers, 2 partial lists, 7 shared thresholds.
 int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float* Ddev, int64_t* Idev, int64_t id_offset, hipStream_t s,
                     unsigned min_ord) {
     const RowStore& R = h->rows;
@@ -141,29 +146,49 @@ int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float*
     for (int64_t done = 0; done < nq; done += kBatch) {
         const int nb = (int)std::min<int64_t>(kBatch, nq - done);
         if (!plan_f8_search(ld, R.nrows, nb, k, h->num_cu, &p)) return fail("internal: 8-bit search plan failed");
-        F8Mat qm{q.codes + done * q.stride, q.stride, q.scales + done * q.sstride, q.sstride, nb};
-        if (q.f32) {
-            const size_t codes = (size_t)nb * ld;
-            CHECK(ensure_ws(h, 4, codes + (size_t)nb * sld));
-            unsigned char* w = (unsigned char*)h->ws[4];
-            HIPCHECK(launch_f8_rows(plain_rows(q.f32 + done * q.q_stride, q.q_stride, SSMI_F32, nb, R.d, w, ld, w + codes, sld), h->num_cu, s));
-            qm = F8Mat{w, ld, w + codes, sld, nb};
-        }
-        CHECK(ensure_ws(h, 2, p.partial_bytes));
-        if (p.cand_bytes) CHECK(ensure_ws(h, 5, p.cand_bytes));
-        if (p.share_bytes) CHECK(ensure_ws(h, 7, p.share_bytes));
-        const size_t i_bytes = (size_t)nb * p.kp * 8;
-        CHECK(ensure_ws(h, 6, i_bytes + (size_t)nb * p.kp * 4));
-        int64_t* I1 = (int64_t*)h->ws[6];
-        float* D1 = (float*)((char*)h->ws[6] + i_bytes);
-        const bool tail = p.scan && h->tail_counters;
-        const TailMerge tm{tail ? h->tail_counters : nullptr, D1, I1, 0, nullptr, nullptr, nullptr, nullptr, 0};
         const bool rec = h->timing_on && done == 0;
-        if (rec) HIPCHECK(hipEventRecord(ev[0], s));
-        HIPCHECK(launch_f8_search(view, qm, k, p, h->ws[7], h->ws[5], (skey_t*)h->ws[2], tm, s));
-        if (rec) HIPCHECK(hipEventRecord(ev[1], s));
-        if (!tail) HIPCHECK(launch_merge_keys((const skey_t*)h->ws[2], nb, p.parts, p.kp, D1, I1, 0, s));
-        HIPCHECK(launch_f8_finish(view, qm, I1, p.kp, k, Ddev + done * k, Idev + done * k, id_offset, min_ord, s));
+        CHECK(ensure_ws(h, 2, p.partial_bytes));
+        F8ScanArgs a = {};
+        a.v = view;
+        a.q = F8Mat{q.codes + done * q.stride, q.stride, q.scales + done * q.sstride, q.sstride, nb};
+        a.f32 = q.f32 ? q.f32 + done * q.q_stride : nullptr;
+        a.f32_stride = q.q_stride;
+        a.f32_vec = ((uintptr_t)a.f32 & 15) == 0 && q.q_stride % 4 == 0;
+        a.d = R.d;
+        a.k = k;
+        a.kp = p.kp;
+        a.partial = (skey_t*)h->ws[2];
+        a.D = Ddev + done * k;
+        a.I = Idev + done * k;
+        a.id_offset = id_offset;
+        a.min_ord = min_ord;
+        a.cap = p.cap;
+        a.every = p.every;
+        if (p.scan) {
+            if (h->tail_counters) {
+                a.counter = nb == 1 ? h->tail_counters : nullptr;
+                a.shared = h->tail_counters + 1;
+            }
+            if (rec) HIPCHECK(hipEventRecord(ev[0], s));
+            HIPCHECK(launch_f8_scan(a, p, s));
+            if (rec) { HIPCHECK(hipEventRecord(ev[1], s)); h->merge_event = false; }
+            if (a.counter) continue;
+        } else {
+            if (q.f32) {
+                const size_t codes = (size_t)nb * ld;
+                CHECK(ensure_ws(h, 4, codes + (size_t)nb * sld));
+                unsigned char* w = (unsigned char*)h->ws[4];
+                HIPCHECK(launch_f8_rows(plain_rows(a.f32, q.q_stride, SSMI_F32, nb, R.d, w, ld, w + codes, sld), h->num_cu, s));
+                a.q = F8Mat{w, ld, w + codes, sld, nb};
+                a.f32 = nullptr;
+            }
+            CHECK(ensure_ws(h, 5, p.cand_bytes));
+            CHECK(ensure_ws(h, 7, p.share_bytes));
+            if (rec) HIPCHECK(hipEventRecord(ev[0], s));
+            HIPCHECK(launch_f8_tiles(view, a.q, p, h->ws[7], h->ws[5], (skey_t*)h->ws[2], s));
+            if (rec) HIPCHECK(hipEventRecord(ev[1], s));
+        }
+        HIPCHECK(launch_f8_finish(a, p, s));
         if (rec) { HIPCHECK(hipEventRecord(ev[2], s)); h->merge_event = true; }
     }
     if (h->timing_on) h->n_searches++;
@@ -172,7 +197,7 @@ int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float*
     h->timing.last_path = p.scan ? 0 : 1;
     h->last_kernel = p.kernel;
     h->last_clk = nullptr;
-    h->timing.last_grid = p.grid_x * p.grid_y;
+    h->timing.last_grid = p.grid_x;
     h->timing.last_scan_bytes = (int64_t)R.nrows * (ld + f8_blocks(R.d));
     h->timing.last_scan_flops = 2ll * std::min<int64_t>(nq, kBatch) * R.nrows * R.d;
     return 0;

@@ -49,29 +49,35 @@ __device__ __forceinline__ void store8(T* row, int e0, int d, const float (&o)[8
     }
 }
 
-// sum over the threads that share a row: a wave (ROWS_PER_BLOCK > 1) or the whole block
+// (a, b) summed over the threads that share a row: a wave, or the whole block
 template <bool WAVE>
-__device__ __forceinline__ float row_sum(float v, float* lds) {
-    v = wave_sum(v);
+__device__ __forceinline__ void row_sums(double& a, double& b, double2* lds) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        a += __shfl_xor(a, d);
+        b += __shfl_xor(b, d);
+    }
     if constexpr (!WAVE) {
         const int nw = (int)(blockDim.x >> 6);
         if (nw > 1) {
-            __syncthreads();  // the words of the previous sum are free
-            if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+            __syncthreads();  // the words of the previous row are free
+            if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = double2{a, b};
             __syncthreads();
-            v = (int)(threadIdx.x & 63) < nw ? lds[threadIdx.x & 63] : 0.f;
-            v = wave_sum(v);
+            a = b = 0.0;
+            for (int w = 0; w < nw; ++w) { a += lds[w].x; b += lds[w].y; }
         }
     }
-    return v;
 }
 
 // Eight elements per thread and pass: 16 threads hold a block of 128, so its maximum is four DPP steps and the codes leave as
-// 8 bytes per lane.  WAVE: a row per wave (rows up to 2048 elements, many of them), else a row per block.  Sums in fp32.
+// 8 bytes per lane.  WAVE: a row per wave (rows up to 2048 elements, many of them), else a row per block.
+// The norm's sums and its one factor per row are 64-bit: y is then the exact value rounded once, and an element's code is that of
+// the exact row unless y lies within 2^-24 of a border.  (With fp32 sums and factors three times as many codes parted from the exact
+// ones; the 64-bit products hide behind memory.)  unit needs no second pass: |y| = f |h w| for y = f h w.
 // (Eight passes of 1024 threads would take rows of 65536 elements through the norm too, but spill.)
-template <typename T, int ITER, bool WAVE, bool VEC>
+template <typename T, int ITER, bool WAVE, bool VEC, bool NORM>
 __global__ void __launch_bounds__(WAVE ? 256 : 1024) f8_rows_kernel(F8NormArgs a) {
-    __shared__ float red[16];
+    __shared__ double2 red[16];
     const int tpr = WAVE ? 64 : (int)blockDim.x;
     const int t = WAVE ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
     const long long step = WAVE ? (long long)gridDim.x * 4 : (long long)gridDim.x;
@@ -83,7 +89,7 @@ __global__ void __launch_bounds__(WAVE ? 256 : 1024) f8_rows_kernel(F8NormArgs a
             float v[ITER][8];
 #pragma unroll
             for (int i = 0; i < ITER; ++i) load8<T, VEC>(x, c0 + (i * tpr + t) * 8, a.d, v[i]);
-            if (a.residual) {
+            if (NORM && a.residual) {
                 const T* r = static_cast<const T*>(a.residual) + row * a.r_stride;
                 T* ro = static_cast<T*>(a.residual_out) + row * a.ro_stride;
 #pragma unroll
@@ -97,77 +103,49 @@ __global__ void __launch_bounds__(WAVE ? 256 : 1024) f8_rows_kernel(F8NormArgs a
                     store8<T, VEC>(ro, c0 + (i * tpr + t) * 8, a.d, v[i]);
                 }
             }
-            if (a.norm) {
-                float ss = 0.f;
-#pragma unroll
-                for (int i = 0; i < ITER; ++i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j], v[i][j], ss);
-                ss = row_sum<WAVE>(ss, red);
-                const float rs = 1.f / sqrtf(ss / (float)a.d + a.eps);
-#pragma unroll
-                for (int i = 0; i < ITER; ++i) {
-                    const int e0 = c0 + (i * tpr + t) * 8;
-                    float w[8];
+            if constexpr (NORM) {
+                auto weights = [&](int e0, float (&w)[8]) {
                     if (a.weight && e0 < a.d) {
                         if (a.weight_dtype == 0) load8<float, VEC>(static_cast<const float*>(a.weight), e0, a.d, w);
                         else if (a.weight_dtype == 1) load8<__half, VEC>(static_cast<const __half*>(a.weight), e0, a.d, w);
                         else load8<bf16_t, VEC>(static_cast<const bf16_t*>(a.weight), e0, a.d, w);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rs * w[j];
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[i][j] *= rs;
+                        for (int j = 0; j < 8; ++j) w[j] = 1.f;
+                    }
+                };
+                double hh = 0.0, yy = 0.0;   // sums of h^2 and (h w)^2
+#pragma unroll
+                for (int i = 0; i < ITER; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) hh = fma((double)v[i][j], (double)v[i][j], hh);
+                    if (a.unit) {
+                        float w[8];
+                        weights(c0 + (i * tpr + t) * 8, w);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const double y = (double)v[i][j] * (double)w[j];
+                            yy = fma(y, y, yy);
+                        }
                     }
                 }
-                if (a.unit) {
-                    float s2 = 0.f;
+                row_sums<WAVE>(hh, yy, red);
+                double f = 1.0 / sqrt(hh / (double)a.d + (double)a.eps);
+                if (a.unit) f /= fmax(f * sqrt(yy), 1e-12);
 #pragma unroll
-                    for (int i = 0; i < ITER; ++i)
+                for (int i = 0; i < ITER; ++i) {
+                    float w[8];
+                    weights(c0 + (i * tpr + t) * 8, w);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) s2 = fmaf(v[i][j], v[i][j], s2);
-                    s2 = row_sum<WAVE>(s2, red);
-                    const float inv = 1.f / fmaxf(sqrtf(s2), 1e-12f);
-#pragma unroll
-                    for (int i = 0; i < ITER; ++i)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) v[i][j] *= inv;
+                    for (int j = 0; j < 8; ++j) v[i][j] = (float)((double)v[i][j] * (double)w[j] * f);
                 }
             }
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
                 const int e0 = c0 + (i * tpr + t) * 8;
-                // largest magnitude of the block as an integer: NaN > infinity > every finite value
-                unsigned m = 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
-                m = max(m, (unsigned)xor_lane<1>((int)m));
-                m = max(m, (unsigned)xor_lane<2>((int)m));
-                m = max(m, (unsigned)xor_lane<4>((int)m));
-                m = max(m, (unsigned)xor_lane<8>((int)m));
+                unsigned b;
+                const uint2 o = f8_pack8(v[i], e0, a.d, b);
                 if (e0 < ld) {
-                    uint2 o;
-                    unsigned b = 255u;
-                    if (m < 0x7f800000u) {
-                        // m = f * 2^(E-127), 1 <= f < 2, and 448 = 1.75 * 2^8
-                        const int be = (int)(m >> 23) - 8 + ((m & 0x7fffffu) > 0x600000u ? 1 : 0);
-                        b = (unsigned)max(be, 0);
-                        const float inv = __uint_as_float((254u - b) << 23);
-                        int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][0] * inv, v[i][1] * inv, 0, false);
-                        lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][2] * inv, v[i][3] * inv, lo, true);
-                        int hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][4] * inv, v[i][5] * inv, 0, false);
-                        hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][6] * inv, v[i][7] * inv, hi, true);
-                        o.x = (unsigned)lo;
-                        o.y = (unsigned)hi;
-                    } else {  // an infinity or a NaN makes its block NaN; the padding keeps its zero codes
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            unsigned w = 0;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) w |= e0 + h * 4 + j < a.d ? 0x7fu << (8 * j) : 0u;
-                            if (h == 0) o.x = w; else o.y = w;
-                        }
-                    }
                     *reinterpret_cast<uint2*>(a.codes + row * a.stride + e0) = o;
                     if ((t & 15) == 0) a.scales[row * a.sstride + e0 / kF8Block] = (unsigned char)b;
                 }
@@ -200,8 +178,9 @@ static hipError_t launch_rows_t(const F8NormArgs& a, int num_cu, hipStream_t s) 
     iter = iter <= 1 ? 1 : iter <= 2 ? 2 : 4;
     const long long blocks = wave ? (a.n + 3) / 4 : a.n;
     const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
-#define GO(I, W, V) hipLaunchKernelGGL((f8_rows_kernel<T, I, W, V>), grid, dim3(threads), 0, s, a)
-#define GO_V(I, W) { if (vec) GO(I, W, true); else GO(I, W, false); }
+#define GO(I, W, V) { if (a.norm) hipLaunchKernelGGL((f8_rows_kernel<T, I, W, V, true>), grid, dim3(threads), 0, s, a); \
+                      else hipLaunchKernelGGL((f8_rows_kernel<T, I, W, V, false>), grid, dim3(threads), 0, s, a); }
+#define GO_V(I, W) { if (vec) GO(I, W, true) else GO(I, W, false) }
     if (wave) { if (iter == 1) GO_V(1, true) else if (iter == 2) GO_V(2, true) else GO_V(4, true) }
     else if (iter == 1) GO_V(1, false)
     else if (iter == 2) GO_V(2, false)

@@ -1,8 +1,8 @@
 // f8_search.hip - Flat search over 8-bit rows (f8.h): the product of f8_tile.h with the top-k epilogues of the other row types.
 //
 // Two passes.  The first keeps, for every query, the best k + 16 rows by the matrix instruction's sums (whose error against
-// the exact sum is about 1e-6 |q||x|): a streaming scan for a few queries, bound by reading the rows once, or the tile kernel
-// with the candidate buffers of the 16-bit kernels (mfma_common.h).  The second sums those candidates' products in 64 bits -
+// the exact sum is about 1e-6 |q||x|): a streaming scan for a few queries, bound by reading the rows once (for one query
+// the whole search is its one launch), or the tile kernel with the candidate buffers of the 16-bit kernels (mfma_common.h).  The second sums those candidates' products in 64 bits -
 // every product of two codes is exact in fp32 and the scales are powers of two, so the sum is exact or off by a rounding of
 // 2^-53 - and sorts them by that, ties by the lower id.  A query therefore gets the same ids and scores in any batch.
 //
@@ -13,163 +13,482 @@
 
 namespace ssmi {
 
-__device__ __forceinline__ uint4 load16_once(const unsigned char* p) {
-    typedef unsigned u4 __attribute__((ext_vector_type(4)));
-    const u4 v = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p));
-    return uint4{v[0], v[1], v[2], v[3]};
+__device__ __forceinline__ i32x4_t load16_once(const unsigned char* p) { return __builtin_nontemporal_load(reinterpret_cast<const i32x4_t*>(p)); }
+
+// ---- second pass of one query: 64-bit scores of its candidates, sorted.  All threads of the workgroup ----
+// Four candidates per wave at a time (their loads travel together: the pass is a chain of memory round trips); the 16 codes of
+// a lane belong to one block, so their products add up in 64 bits unscaled and meet the block's scale once.  score / cid: kp
+// words of LDS each.
+//
+// The sum of 16 products without a 64-bit operation for each: a product is a multiple of 2^-18 below 2^18.  S, near 1.5 * 2^23,
+// takes its whole part (an fp32 add there rounds to whole numbers, and 16 products keep S between 2^23 and 2^24), L what the
+// rounding left: at most 1/2 each, so their sum is exact in fp32 too.
+__device__ __forceinline__ double dot16(const i32x4_t& x, const i32x4_t& y) {
+    const float S0 = 12582912.f;   // 1.5 * 2^23
+    float S = S0, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        float a[4], b[4];
+        f8_unpack4((unsigned)x[w], a);
+        f8_unpack4((unsigned)y[w], b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float s = __fmaf_rn(a[j], b[j], S);
+            L = __fadd_rn(L, __fmaf_rn(a[j], b[j], __fsub_rn(S, s)));
+            S = s;
+        }
+    }
+    return (double)__fsub_rn(S, S0) + (double)L;
 }
-__device__ __forceinline__ i32x8_t frag(const uint4& lo, const uint4& hi) {
-    return i32x8_t{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+__device__ __forceinline__ void finish_query(const F8View& V, const unsigned char* qc, const unsigned char* qsc, const int64_t* ids, int kp, int k,
+                                             float* D, int64_t* I, int64_t id_offset, unsigned min_ord, double* score, int64_t* cid) {
+    constexpr int N = 4;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), nwaves = blockDim.x >> 6;
+    const long long seg_mask = (1ll << V.X.seg_shift) - 1;
+    for (int c0 = wave * N; c0 < kp; c0 += nwaves * N) {
+        const unsigned char* xc[N];
+        const unsigned char* xs[N];
+        int64_t id[N];
+        double sum[N];
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            id[t] = c0 + t < kp ? ids[c0 + t] : -1;
+            const long long row = id[t] < 0 ? 0 : id[t], seg = row >> V.X.seg_shift, off = row & seg_mask;   // none: row 0, not used
+            xc[t] = static_cast<const unsigned char*>(V.X.segs[seg]) + off * V.X.ld;
+            xs[t] = static_cast<const unsigned char*>(V.ssegs[seg]) + off * V.sld;
+            sum[t] = 0.0;
+        }
+#pragma unroll 4
+        for (int e = lane * 16; e < V.X.ld; e += 1024) {
+            const int blk = e / kF8Block;
+            i32x4_t x[N];
+            unsigned char sx[N];
+#pragma unroll
+            for (int t = 0; t < N; ++t) {
+                x[t] = *reinterpret_cast<const i32x4_t*>(xc[t] + e);
+                sx[t] = xs[t][blk];
+            }
+            const i32x4_t y = *reinterpret_cast<const i32x4_t*>(qc + e);
+            const double sq = (double)f8_scale(qsc[blk]);
+#pragma unroll
+            for (int t = 0; t < N; ++t) sum[t] += dot16(x[t], y) * (sq * (double)f8_scale(sx[t]));
+        }
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+#pragma unroll
+            for (int d = 32; d >= 1; d >>= 1) sum[t] += __shfl_xor(sum[t], d);
+            if (lane == 0 && c0 + t < kp) {
+                score[c0 + t] = sum[t];
+                cid[c0 + t] = id[t] >= 0 && sum[t] == sum[t] ? id[t] : -1;   // a NaN is no result
+            }
+        }
+    }
+    __syncthreads();
+    // a wave ranks one candidate at a time against 64 others per step
+    int valid = 0;
+    for (int o = lane; o - lane < kp; o += 64) valid += __builtin_popcountll(__builtin_amdgcn_ballot_w64(o < kp && cid[o < kp ? o : 0] >= 0));
+    for (int c = wave; c < kp; c += nwaves) {
+        const int64_t id = cid[c];
+        if (id < 0) continue;
+        const double s = score[c];
+        int rank = 0;
+        for (int o = lane; o - lane < kp; o += 64) {
+            const int oc = o < kp ? o : 0;
+            const double so = score[oc];
+            const int64_t io = cid[oc];
+            rank += __builtin_popcountll(__builtin_amdgcn_ballot_w64(o < kp && io >= 0 && (so > s || (so == s && io < id))));
+        }
+        if (lane == 0 && rank < k) {
+            const float f = (float)s;
+            const bool keep = f32_to_ord(f) >= min_ord;   // the score floor cuts a suffix of the sorted list
+            D[rank] = keep ? f : SSMI_NEG_MAX;
+            I[rank] = keep ? id + id_offset : -1;
+        }
+    }
+    for (int c = valid + threadIdx.x; c < k; c += blockDim.x) { D[c] = SSMI_NEG_MAX; I[c] = -1; }
 }
 
-// ---- streaming scan: up to BT <= 8 queries per launch row, 16 rows per wave pass ----
-// The instruction's sixteen columns cost nothing here (a row of 4096 codes is 1/16 of 32 instructions against 4 KiB of
-// memory); columns beyond BT repeat a query and are never looked at.  Rows go straight into registers: four blocks (512
-// codes) of 16 rows per stage = eight 16-byte loads per lane, two stages in flight.  Queries sit in LDS, rows of ld + 16 bytes
-// so that the 16 lanes of a pass hit 16 different bank groups.
-template <int BT, int R>
-__global__ void __launch_bounds__(512) f8_scan_kernel(F8View V, F8Mat q, int k, skey_t* partial, TailMerge tail) {
+// ---- between the passes: the first pass's lists of one query -> its kp best rows.  All threads of the workgroup ----
+// The lists' m-th keys, m = ceil(kp / P), bound the kp-th best from below: if c = ceil(kp / m) of them reach a score, m c >= kp
+// rows do.  (For kp <= 48 the lane maxima of the heads serve, 64 values instead of P.)  The keys at or above the bound, two or
+// three times kp of the P kp, are collected and sorted.  A full merge of 256 lists of 216 keys took 100 us on one workgroup.
+// keys: LDS, nwaves * 64 R words and at least kSurvivors + 2; ids: kp words of LDS.
+static constexpr int kSurvivors = 2048;
+template <int RV>
+__device__ __forceinline__ unsigned nth_score(const skey_t* lists, int P, int kp, int m, int c) {
+    const int lane = lane_id();
+    WaveSort32<RV> t;
+#pragma unroll
+    for (int r = 0; r < RV; ++r) {
+        const int p = r * 64 + lane;
+        t.v[r] = p < P ? (unsigned)(load_key<true>(lists + (size_t)p * kp + m - 1) >> 32) : 0u;
+    }
+    t.sort_desc();
+    return t.kth(c);
+}
+template <int R>
+__device__ __forceinline__ void merge_to_ids(const skey_t* lists, int P, int kp, skey_t* keys, int64_t* ids) {
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), nwaves = blockDim.x >> 6;
+    unsigned* word = reinterpret_cast<unsigned*>(keys);   // [0] bound, [1] survivors
+    skey_t* surv = keys + 1;
+    const int total = P * kp;
+    WaveTopK<R> t;
+    t.init();
+    // the first keys of every thread travel while wave 0 finds the bound
+    skey_t key[4];
+    auto load4 = [&](int e0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int e = e0 + j * (int)blockDim.x;
+            key[j] = e < total ? load_key<true>(lists + e) : 0;
+        }
+    };
+    load4(threadIdx.x);
+    if (wave == 0) {
+        unsigned bound = 0;
+        const int m = (kp + P - 1) / P, c = (kp + m - 1) / m;
+        if (kp <= 48 && P > 64) {
+            WaveSort32<1> h;
+            h.v[0] = 0;
+            for (int p = lane; p < P; p += 64) h.v[0] = max(h.v[0], (unsigned)(load_key<true>(lists + (size_t)p * kp) >> 32));
+            h.sort_desc();
+            bound = h.kth(kp);
+        } else if (P <= 64) bound = nth_score<1>(lists, P, kp, m, c);
+        else if (P <= 128) bound = nth_score<2>(lists, P, kp, m, c);
+        else if (P <= 256) bound = nth_score<4>(lists, P, kp, m, c);
+        else if (P <= 512) bound = nth_score<8>(lists, P, kp, m, c);
+        if (lane == 0) { word[0] = bound; word[1] = 0; }
+    }
+    __syncthreads();
+    const unsigned bound = max(word[0], 1u);   // (0 is the score of an empty key)
+    for (int e0 = threadIdx.x;;) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if ((unsigned)(key[j] >> 32) >= bound) {
+                const unsigned pos = atomicAdd(word + 1, 1u);
+                if (pos < (unsigned)kSurvivors) surv[pos] = key[j];
+            }
+        e0 += blockDim.x * 4;
+        if (e0 >= total) break;
+        load4(e0);
+    }
+    __syncthreads();
+    const int n = (int)word[1];
+    if (n <= kSurvivors) {
+        for (int base = wave * 64; base < n; base += nwaves * 64) {
+            WaveTopK<1> c;
+            c.v[0] = base + lane < n ? surv[base + lane] : 0;
+            c.sort_desc();
+            t.merge_regs(c);
+        }
+    } else {   // the bound did not thin them: every key
+        for (int base = wave * 64; base < total; base += nwaves * 64) {
+            WaveTopK<1> c;
+            c.v[0] = base + lane < total ? load_key<true>(lists + base + lane) : 0;
+            if (__builtin_amdgcn_ballot_w64(c.v[0] > t.kth(kp)) == 0) continue;
+            c.sort_desc();
+            t.merge_regs(c);
+        }
+    }
+    __syncthreads();
+    block_merge<R>(t, keys, wave, nwaves);
+    if (wave == 0) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int e = r * 64 + lane;
+            if (e < kp) ids[e] = t.v[r] ? (int64_t)key_id(t.v[r]) : -1;
+        }
+    }
+    __syncthreads();
+}
+__host__ __device__ inline size_t merge_keys_bytes(int waves, int r) {
+    const size_t a = (size_t)waves * 64 * r * sizeof(skey_t), b = (size_t)(kSurvivors + 2) * sizeof(skey_t);
+    return a > b ? a : b;
+}
+
+// query b -> LDS, quantised on the way if it comes as fp32 (16 lanes hold a block).  All threads of the workgroup
+__device__ __forceinline__ void stage_query(const F8ScanArgs& A, long long b, unsigned char* qs, unsigned char* qsc) {
+    for (int c = threadIdx.x; c < A.v.X.ld / 8; c += blockDim.x) {
+        const int e0 = c * 8;
+        uint2 o;
+        unsigned sb = 0;
+        if (A.f32) {
+            const float* src = A.f32 + b * A.f32_stride;
+            float v[8];
+            if (A.f32_vec && e0 + 8 <= A.d) {
+                const float4 lo = *reinterpret_cast<const float4*>(src + e0), hi = *reinterpret_cast<const float4*>(src + e0 + 4);
+                v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+                v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = e0 + j < A.d ? src[e0 + j] : 0.f;
+            }
+            o = f8_pack8(v, e0, A.d, sb);
+        } else {
+            o = *reinterpret_cast<const uint2*>(A.q.codes + b * A.q.stride + e0);
+            sb = A.q.scales[b * A.q.sstride + e0 / kF8Block];
+        }
+        *reinterpret_cast<uint2*>(qs + e0) = o;
+        if ((e0 & (kF8Block - 1)) == 0) qsc[e0 / kF8Block] = (unsigned char)sb;
+    }
+}
+
+// what follows the first pass where it does not carry it: one workgroup per query
+template <int R>
+__global__ void __launch_bounds__(1024) f8_finish_kernel(F8ScanArgs A, int P) {
     extern __shared__ __align__(16) unsigned char smem[];
+    const long long qi = blockIdx.x;
+    const int ld = A.v.X.ld, kp = A.kp;
+    unsigned char* qs = smem;
+    unsigned char* qsc = smem + ld;
+    skey_t* keys = reinterpret_cast<skey_t*>(smem + (ld + ld / kF8Block + 15) / 16 * 16);
+    double* score = reinterpret_cast<double*>(reinterpret_cast<unsigned char*>(keys) + merge_keys_bytes(blockDim.x >> 6, R));
+    int64_t* cid = reinterpret_cast<int64_t*>(score + kp);
+    int64_t* ids = cid + kp;
+    if (A.shared && threadIdx.x == 0) A.shared[qi] = 0;   // as the next launch expects it
+    stage_query(A, qi, qs, qsc);
+    merge_to_ids<R>(A.partial + (size_t)qi * P * kp, P, kp, keys, ids);
+    finish_query(A.v, qs, qsc, ids, kp, A.k, A.D + qi * A.k, A.I + qi * A.k, A.id_offset, A.min_ord, score, cid);
+}
+
+// ---- streaming scan: up to BT <= 8 queries ----
+// Bound by reading the rows once; what reads fastest decides the layout.  A plain read of 1M x 4096 codes ran at 5.9 TB/s with
+// 16 rows x 64 bytes per load instruction (the operand layout of the 16x16x128 instruction as it is) and at 6.7-7.0 TB/s with 8
+// rows x 128 bytes, non-temporal loads and 4-8 waves per CU.  So one load is one whole block of eight rows, 16 codes a lane,
+// and feeds the low half of one instruction whose high half is zero (the matrix pipe is 7 % busy): the sixteen operand rows
+// are the 8 rows x {even, odd 16-byte chunks}, the sixteen columns 8 queries x {even, odd chunks}, and a score is the
+// sum of the even-even and the odd-odd element of the result.  Columns beyond BT repeat a query and are never looked at.
+// Up to eight loads (8 KiB) per stage and wave, three stages in flight: NB = 0: a stage is up to eight blocks of one group of
+// eight rows; NB = 1, 2, 4: rows of that many blocks, a stage is 8 / NB groups;
+// NB = 8: rows of a multiple of eight blocks, every stage is whole.
+//
+// Lists are the workgroup's: scores at or above a query's threshold go to its candidate buffer in LDS, and at looks ever
+// further apart one wave per query sorts the buffer into the query's list (topk.h), which raises the threshold; the workgroups
+// share the highest one.  (A list per wave, one sorted insertion per candidate, took longer than the rows for eight
+// queries: a wave sees 500 of 1M rows, so its lists of k + 16 are never warm.)
+template <int BT, int R, int NB>
+__global__ void __launch_bounds__(512) f8_scan_kernel(F8ScanArgs A) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    const F8View& V = A.v;
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int nwaves = (int)(blockDim.x >> 6);
-    const int ld = V.X.ld, nblk = ld / kF8Block, nst = (nblk + 3) / 4;
-    const int q0 = blockIdx.y * BT, nq = (int)q.n;
-    const int qpitch = ld + 16;
-    unsigned char* qs = smem;
-    int* qsc = reinterpret_cast<int*>(smem + BT * qpitch);   // [BT][nst] words of four scales
-    for (int b = 0; b < BT; ++b) {
-        const long long qi = min(q0 + b, nq - 1);
-        for (int e = threadIdx.x * 16; e < ld; e += blockDim.x * 16)
-            *reinterpret_cast<uint4*>(qs + b * qpitch + e) = *reinterpret_cast<const uint4*>(q.codes + qi * q.stride + e);
-        for (int e = threadIdx.x; e < nst; e += blockDim.x) qsc[b * nst + e] = *reinterpret_cast<const int*>(q.scales + qi * q.sstride + e * 4);
+    const int ld = V.X.ld, nblk = ld / kF8Block, nq = (int)A.q.n, kp = A.kp;
+    const int qpitch = ld + 32;                              // the 16 lanes of a pass (8 queries x 2 chunks) cover all banks once
+    const int spitch = (nblk + 7) / 8 * 8;
+    unsigned char* qs = smem;                                // [BT][qpitch] codes
+    unsigned char* qsc = smem + BT * qpitch;                 // [BT][spitch] scales
+    float* thr_l = reinterpret_cast<float*>(smem + (BT * (qpitch + spitch) + 15) / 16 * 16);   // [8] thresholds
+    unsigned* cnt_l = reinterpret_cast<unsigned*>(thr_l + 8);                                   // [8] candidates
+    skey_t* kept = reinterpret_cast<skey_t*>(cnt_l + 8);     // [BT][64 R] lists, best first
+    skey_t* cand = kept + BT * 64 * R;                       // [BT][A.cap] candidates; the tail's scratch after that
+    for (int e = threadIdx.x; e < BT * 64 * R; e += blockDim.x) kept[e] = 0;
+    // a score passes only at or above its query's threshold, and NaN never does; queries that only fill up BT pass nothing
+    if (threadIdx.x < 8) {
+        thr_l[threadIdx.x] = (int)threadIdx.x < min(BT, nq) ? -__builtin_inff() : __builtin_nanf("");
+        cnt_l[threadIdx.x] = 0;
     }
-    __syncthreads();
 
-    WaveTopK<R> top[BT];
-    skey_t thr[BT];
-#pragma unroll
-    for (int b = 0; b < BT; ++b) { top[b].init(); thr[b] = 0; }
-    const int col = lane & 15, grp = lane >> 4;
-    // a score passes only at or above the gate of its lane's query; NaN never does.  Columns that repeat a query are shut
-    float gate = col < BT ? -__builtin_inff() : __builtin_nanf("");
-
+    const int r8 = lane & 7, odd = (lane >> 3) & 1, grp = lane >> 4;
+    const bool holds = (lane & 40) == 0;   // scores end up in the lanes with bits 3 and 5 clear
     const unsigned vb = (gridDim.x % 8 == 0) ? (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
-    const long long ngroups = (V.X.nrows + 15) >> 4, step = (long long)gridDim.x * nwaves;
+    constexpr int G = NB == 0 ? 1 : 8 / (NB == 0 ? 1 : NB);   // groups of eight rows per run
+    constexpr int run_rows = G * 8;
+    const long long nruns = (V.X.nrows + run_rows - 1) / run_rows, step = (long long)gridDim.x * nwaves;
     const long long seg_mask = (1ll << V.X.seg_shift) - 1;
-    const unsigned char* qlane = qs + (col % BT) * qpitch + grp * 16;
-    const int* qslane = qsc + (col % BT) * nst;
+    const int chunk = (2 * grp + odd) * 16;
+    const unsigned lane_off = (unsigned)r8 * (unsigned)ld + chunk, lane_soff = (unsigned)r8 * (unsigned)V.sld;
+    const unsigned char* qlane = qs + (r8 % BT) * qpitch + chunk;
+    const unsigned char* qslane = qsc + (r8 % BT) * spitch;
+    const int stages = NB && NB < 8 ? 1 : (nblk + 7) / 8;     // of a run
 
-    struct Base { const unsigned char* c; const unsigned char* s; };
-    auto group_base = [&](long long g) -> Base {
-        long long row = (g << 4) + col;   // 16 rows of a group share a segment; beyond the last row: the last
-        if (row >= V.X.nrows) row = V.X.nrows - 1;
-        const long long seg = (g << 4) >> V.X.seg_shift, off = row & seg_mask;
-        return Base{static_cast<const unsigned char*>(V.X.segs[seg]) + off * ld + grp * 16, static_cast<const unsigned char*>(V.ssegs[seg]) + off * V.sld};
+    // two cursors over the wave's stages: the next to load, and the next to multiply.  A run's rows share a segment, and a
+    // segment holds whole runs: rows beyond the last are read, never offered to a list
+    long long lrun = (long long)vb * nwaves + wave, crun = lrun;
+    int lkb = 0, ckb = 0;                                     // first block of the stage
+    const unsigned char *lc = nullptr, *ls = nullptr;         // the run's codes and scales
+    auto aim = [&]() __attribute__((always_inline)) {
+        const long long row = lrun * run_rows, seg = row >> V.X.seg_shift, off = row & seg_mask;
+        lc = static_cast<const unsigned char*>(V.X.segs[seg]) + off * ld;
+        ls = static_cast<const unsigned char*>(V.ssegs[seg]) + off * V.sld;
     };
-    uint4 xa[8], xb[8];
-    int sa = 0, sb = 0;
-    auto load = [&](uint4 (&x)[8], int& sc, const Base& p, int st) {
-        sc = *reinterpret_cast<const int*>(p.s + st * 4);
+    if (lrun < nruns) aim();
+    auto fetch = [&](i32x4_t (&x)[8], int (&sc)[8]) __attribute__((always_inline)) {
+        if (lrun >= nruns) return;
+        if constexpr (NB == 0 || NB == 8) {
+            const i32x2_t w = *reinterpret_cast<const i32x2_t*>(ls + lkb + lane_soff);   // (scale rows are multiples of 16 bytes)
+            sc[0] = w[0];
+            sc[1] = w[1];
+            const unsigned char* p = lc + (size_t)lkb * kF8Block + lane_off;
+            // (a stage that is not whole loads its last block again: branches around loads cost more than those)
+            const int last = NB == 8 ? 7 : nblk - 1 - lkb;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int kb = min(st * 4 + j, nblk - 1);   // (a block beyond the row is loaded as the last and not used)
-            x[2 * j] = load16_once(p.c + (size_t)kb * 128);
-            x[2 * j + 1] = load16_once(p.c + (size_t)kb * 128 + 64);
-        }
-    };
-    long long g = (long long)vb * nwaves + wave;
-    if (g >= ngroups) g = -1;
-    Base base = {nullptr, nullptr};
-    if (g >= 0) { base = group_base(g); load(xa, sa, base, 0); }
-    while (g >= 0) {
-        const long long gn = g + step < ngroups ? g + step : -1;
-        const Base next = gn < 0 ? base : group_base(gn);
-        f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        auto consume = [&](const uint4 (&x)[8], int sc, int st) {
-            const int sq = qslane[st];
-            const unsigned char* ql = qlane + (size_t)st * 512;
-            const auto one = [&](auto jc) {
-                constexpr int J = decltype(jc)::value;
-                if (st * 4 + J < nblk) {
-                    const uint4 lo = *reinterpret_cast<const uint4*>(ql + J * 128), hi = *reinterpret_cast<const uint4*>(ql + J * 128 + 64);
-                    acc = mfma_f8<J>(frag(x[2 * J], x[2 * J + 1]), frag(lo, hi), acc, sc, sq);
-                }
-            };
-            one(std::integral_constant<int, 0>());
-            one(std::integral_constant<int, 1>());
-            one(std::integral_constant<int, 2>());
-            one(std::integral_constant<int, 3>());
-        };
-#pragma unroll 1
-        for (int st = 0; st < nst; st += 2) {
-            const bool second = st + 1 < nst;
-            if (second) load(xb, sb, base, st + 1);
-            else load(xb, sb, next, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            consume(xa, sa, st);
-            __builtin_amdgcn_sched_barrier(0);
-            if (second) {
-                if (st + 2 < nst) load(xa, sa, base, st + 2);
-                else load(xa, sa, next, 0);
-                __builtin_amdgcn_sched_barrier(0);
-                consume(xb, sb, st + 1);
-                __builtin_amdgcn_sched_barrier(0);
-            } else {   // odd number of stages: the next group's first stage is in xb
-                sa = sb;
+            for (int j = 0; j < 8; ++j) x[j] = load16_once(p + (NB == 8 ? j : min(j, last)) * kF8Block);
+        } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) xa[j] = xb[j];
+            for (int g = 0; g < G; ++g) {
+                sc[g] = *reinterpret_cast<const int*>(ls + (size_t)(g * 8) * V.sld + lane_soff);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) x[g * NB + j] = load16_once(lc + lane_off + (g * 8 * NB + j) * kF8Block);
             }
         }
-        // acc[i] of lane (col, grp): row 4 grp + i of the group against query col
-        const long long row0 = g << 4;
+        lkb += 8;
+        if ((NB && NB < 8) || lkb >= nblk) {
+            lkb = 0;
+            lrun += step;
+            if (lrun < nruns) aim();
+        }
+    };
+    i32x4_t xa[8], xb[8], xc[8];
+    int sa[8], sb[8], sc[8];
+    fetch(xa, sa);   // the first rows travel while the queries are made
+    fetch(xb, sb);
+    for (int b = 0; b < BT; ++b) stage_query(A, min(b, nq - 1), qs + b * qpitch, qsc + b * spitch);
+
+    f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const i32x4_t zero = i32x4_t{0, 0, 0, 0};
+    // a row group is complete: rows 4 ((lane >> 4) & 1) + i of it, even-even here, odd-odd in lane ^ 40
+    auto offer = [&](int g) __attribute__((always_inline)) {
+        float sum[4];
         bool any = false;
+        const float thr = thr_l[r8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) any |= acc[i] >= gate;
-        if (__builtin_amdgcn_ballot_w64(any) != 0) {
+        for (int i = 0; i < 4; ++i) {
+            sum[i] = acc[i] + __int_as_float(xor_lane<32>(xor_lane<8>(__float_as_int(acc[i]))));
+            any |= sum[i] >= thr;
+        }
+        acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (__builtin_amdgcn_ballot_w64(any && holds) == 0) return;
+        const long long row0 = crun * run_rows + g * 8 + 4 * grp;   // (grp < 2 in the lanes that hold)
+        if (holds) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                unsigned long long mask = __builtin_amdgcn_ballot_w64(acc[i] >= gate);
-                while (mask) {
-                    const int src = (int)__builtin_ctzll(mask);
-                    mask &= mask - 1;
-                    const long long row = row0 + 4 * (src >> 4) + i;
-                    if (row >= V.X.nrows) continue;
-                    const int qb = src & 15;
-                    const skey_t key = make_key(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(acc[i]), src)), (uint32_t)row);
+            for (int i = 0; i < 4; ++i)
+                if (sum[i] >= thr && row0 + i < V.X.nrows) cand[r8 * A.cap + atomicAdd(&cnt_l[r8], 1u)] = make_key(sum[i], (uint32_t)(row0 + i));
+        }
+    };
+    auto eat = [&](const i32x4_t (&x)[8], const int (&sc)[8]) __attribute__((always_inline)) {
+        if (crun >= nruns) return;
+        if constexpr (NB == 0 || NB == 8) {
+            const i32x2_t sq = *reinterpret_cast<const i32x2_t*>(qslane + ckb);
+            const unsigned char* qp = qlane + (size_t)ckb * kF8Block;
+            const auto one = [&](auto jc) __attribute__((always_inline)) {
+                constexpr int J = decltype(jc)::value;
+                const i32x4_t y = *reinterpret_cast<const i32x4_t*>(qp + J * kF8Block);
+                acc = mfma_f8<J % 4>(join8(x[J], zero), join8(y, zero), acc, sc[J / 4], sq[J / 4]);
+            };
+            const int left = nblk - ckb;   // (the rest of a row that is not whole stages)
+            one(std::integral_constant<int, 0>());
+            if (NB == 8 || left > 1) one(std::integral_constant<int, 1>());
+            if (NB == 8 || left > 2) one(std::integral_constant<int, 2>());
+            if (NB == 8 || left > 3) one(std::integral_constant<int, 3>());
+            if (NB == 8 || left > 4) one(std::integral_constant<int, 4>());
+            if (NB == 8 || left > 5) one(std::integral_constant<int, 5>());
+            if (NB == 8 || left > 6) one(std::integral_constant<int, 6>());
+            if (NB == 8 || left > 7) one(std::integral_constant<int, 7>());
+            ckb += 8;
+            if (ckb < nblk) return;
+            ckb = 0;
+            offer(0);
+        } else {
+            const int sq = *reinterpret_cast<const int*>(qslane);
+            i32x4_t y[NB];
 #pragma unroll
-                    for (int b = 0; b < BT; ++b) {
-                        if (b == qb && key > thr[b]) {
-                            top[b].insert(key);
-                            thr[b] = top[b].kth(k);
-                            if (thr[b] && col == b) gate = key_score(thr[b]);
-                        }
-                    }
-                }
+            for (int j = 0; j < NB; ++j) y[j] = *reinterpret_cast<const i32x4_t*>(qlane + j * kF8Block);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                acc = mfma_f8<0>(join8(x[g * NB], zero), join8(y[0], zero), acc, sc[g], sq);
+                if constexpr (NB > 1) acc = mfma_f8<1>(join8(x[g * NB + 1], zero), join8(y[1], zero), acc, sc[g], sq);
+                if constexpr (NB > 2) acc = mfma_f8<2>(join8(x[g * NB + 2], zero), join8(y[2], zero), acc, sc[g], sq);
+                if constexpr (NB > 3) acc = mfma_f8<3>(join8(x[g * NB + 3], zero), join8(y[3], zero), acc, sc[g], sq);
+                offer(g);
             }
         }
-        g = gn;
-        base = next;
-    }
-
-    __syncthreads();
-    skey_t* lds_keys = reinterpret_cast<skey_t*>(smem);
-#pragma unroll
-    for (int b = 0; b < BT; ++b) {
-        block_merge<R>(top[b], lds_keys, wave, nwaves);
-        if (wave == 0 && q0 + b < nq) publish_list<R>(top[b], partial + ((size_t)(q0 + b) * gridDim.x + blockIdx.x) * k, k);
-        __syncthreads();
-    }
-    if (tail.counter == nullptr) return;
-    if (!tail_last_block(tail.counter + blockIdx.y, gridDim.x, reinterpret_cast<unsigned*>(smem))) return;
+        crun += step;
+    };
+    // LDS of every wave settled, loads in flight left alone
+    auto meet = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // candidates of query b -> its list, by the wave that owns b
+    auto fold = [&](bool share) __attribute__((always_inline)) {
 #pragma unroll 1
-    for (int b = 0; b < BT; ++b) {
-        const int qi = q0 + b;
-        if (qi >= nq) break;
-        merge_partials<R, true>(partial + (size_t)qi * gridDim.x * k, (int)gridDim.x, k, lds_keys, wave, nwaves, tail.D + (size_t)qi * k,
-                                tail.I + (size_t)qi * k, 0);
-        __syncthreads();
+        for (int b = wave; b < min(BT, nq); b += nwaves) {
+            const int n = (int)cnt_l[b];
+            if (n == 0) continue;
+            WaveTopK<R> t;
+#pragma unroll
+            for (int r = 0; r < R; ++r) t.v[r] = kept[b * 64 * R + r * 64 + lane];
+#pragma unroll 1
+            for (int base = 0; base < n; base += 64) {
+                WaveTopK<1> c;
+                c.v[0] = base + lane < n ? cand[b * A.cap + base + lane] : 0;
+                if (__builtin_amdgcn_ballot_w64(c.v[0] > t.kth(kp)) == 0) continue;
+                c.sort_desc();
+                t.merge_regs(c);
+            }
+            const skey_t kth = t.kth(kp);
+            t.store(kept + b * 64 * R, 64 * R);
+            if (lane == 0) {
+                cnt_l[b] = 0;
+                // the kp-th score of any workgroup bounds the final one: all filter with the highest
+                unsigned mine = kth ? (unsigned)(kth >> 32) : 0u;
+                if (share && A.shared) mine = max(mine, atomicMax(A.shared + b, mine));
+                if (mine) thr_l[b] = ord_to_f32(mine);
+            }
+        }
+    };
+    const long long rounds = ((long long)vb * nwaves < nruns) ? (nruns - (long long)vb * nwaves + step - 1) / step : 0;
+    const long long total = rounds * stages;   // the same for all waves of the workgroup (wave 0 has the most runs), so that they meet
+    int turns = 0, every = 1;
+    meet();
+    // (the scheduler would otherwise sink every load to its first use)
+#define TURN(X, SX, Y, SY)                  \
+    fetch(Y, SY);                           \
+    __builtin_amdgcn_sched_barrier(0);      \
+    eat(X, SX);                             \
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+    for (long long i = 0; i < total; i += 3) {
+        TURN(xa, sa, xc, sc)
+        TURN(xb, sb, xa, sa)
+        TURN(xc, sc, xb, sb)
+        if (++turns == every && i + 3 < total) {   // (the end folds anyway)
+            // look at the buffers, often while the thresholds are young
+            turns = 0;
+            every = min(2 * every, A.every);
+            meet();
+            bool fill = false;
+#pragma unroll
+            for (int b = 0; b < BT; ++b) fill |= cnt_l[b] >= 64u;
+            meet();   // everybody has looked before a wave clears a counter or appends
+            if (fill) {
+                fold(true);
+                meet();
+            }
+        }
     }
+#undef TURN
+    __syncthreads();
+    fold(false);
+    // publication, and in the last workgroup to arrive the merge (tail_merge.h) and the second pass
+    for (int b = wave; b < nq; b += nwaves) {
+        WaveTopK<R> t;
+#pragma unroll
+        for (int r = 0; r < R; ++r) t.v[r] = kept[b * 64 * R + r * 64 + lane];
+        publish_list<R>(t, A.partial + ((size_t)b * gridDim.x + blockIdx.x) * kp, kp);
+    }
+    if (A.counter == nullptr) return;
+    skey_t* keys = cand;
+    if (!tail_last_block(A.counter, gridDim.x, reinterpret_cast<unsigned*>(keys))) return;
+    // one query: the last workgroup goes on (several queries have a workgroup each: f8_finish_kernel)
+    if (threadIdx.x == 0) A.shared[0] = 0;   // as the next launch expects it
+    double* score = reinterpret_cast<double*>(reinterpret_cast<unsigned char*>(keys) + merge_keys_bytes(nwaves, R));
+    int64_t* cid = reinterpret_cast<int64_t*>(score + kp);
+    int64_t* ids = cid + kp;
+    merge_to_ids<R>(A.partial, (int)gridDim.x, kp, keys, ids);
+    finish_query(V, qs, qsc, ids, kp, A.k, A.D, A.I, A.id_offset, A.min_ord, score, cid);
 }
 
 // ---- tile kernel: 256 rows x TQ queries per workgroup, a slice of the rows each ----
@@ -243,79 +562,7 @@ __global__ void f8_zero_kernel(unsigned* p, int n) {
     if (i < n) p[i] = 0;
 }
 
-// ---- second pass: 64-bit scores of the candidates, sorted ----
-// One workgroup per query, a wave per candidate.  16 codes of a lane belong to one block, so its products add up in 64 bits
-// unscaled and meet the block's scale once.
-__global__ void __launch_bounds__(1024) f8_finish_kernel(F8View V, F8Mat q, const int64_t* __restrict__ ids, int kp, int k, float* D,
-                                                         int64_t* I, int64_t id_offset, unsigned min_ord) {
-    __shared__ double score[kMaxK];
-    __shared__ int64_t cid[kMaxK];
-    __shared__ int nvalid;
-    const int lane = lane_id(), wave = threadIdx.x >> 6, nwaves = blockDim.x >> 6;
-    const long long qi = blockIdx.x;
-    const unsigned char* qc = q.codes + qi * q.stride;
-    const unsigned char* qsc = q.scales + qi * q.sstride;
-    const long long seg_mask = (1ll << V.X.seg_shift) - 1;
-    if (threadIdx.x == 0) nvalid = 0;
-    __syncthreads();
-    for (int c = wave; c < kp; c += nwaves) {
-        const int64_t id = ids[qi * kp + c];
-        double sum = 0.0;
-        if (id >= 0) {
-            const long long seg = id >> V.X.seg_shift, off = id & seg_mask;
-            const unsigned char* xc = static_cast<const unsigned char*>(V.X.segs[seg]) + off * V.X.ld;
-            const unsigned char* xs = static_cast<const unsigned char*>(V.ssegs[seg]) + off * V.sld;
-            for (int e = lane * 16; e < V.X.ld; e += 1024) {
-                const uint4 x = *reinterpret_cast<const uint4*>(xc + e), y = *reinterpret_cast<const uint4*>(qc + e);
-                const unsigned xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
-                double part = 0.0;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    float a[4], b[4];
-                    f8_unpack4(xw[w], a);
-                    f8_unpack4(yw[w], b);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) part += (double)(a[j] * b[j]);
-                }
-                const int blk = e / kF8Block;
-                sum += part * ((double)f8_scale(xs[blk]) * (double)f8_scale(qsc[blk]));
-            }
-        }
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
-        if (lane == 0) {
-            const bool ok = id >= 0 && sum == sum;
-            score[c] = sum;
-            cid[c] = ok ? id : -1;
-            if (ok) atomicAdd(&nvalid, 1);
-        }
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < kp; c += blockDim.x) {
-        const int64_t id = cid[c];
-        if (id < 0) continue;
-        const double s = score[c];
-        int rank = 0;
-        for (int o = 0; o < kp; ++o) rank += cid[o] >= 0 && (score[o] > s || (score[o] == s && cid[o] < id)) ? 1 : 0;
-        if (rank < k) {
-            const float f = (float)s;
-            const bool keep = f32_to_ord(f) >= min_ord;   // the score floor cuts a suffix of the sorted list
-            D[qi * k + rank] = keep ? f : SSMI_NEG_MAX;
-            I[qi * k + rank] = keep ? id + id_offset : -1;
-        }
-    }
-    for (int c = nvalid + threadIdx.x; c < k; c += blockDim.x) { D[qi * k + c] = SSMI_NEG_MAX; I[qi * k + c] = -1; }
-}
-
-hipError_t launch_f8_finish(const F8View& v, const F8Mat& q, const int64_t* ids, int kp, int k, float* D, int64_t* I,
-                            int64_t id_offset, unsigned min_ord, hipStream_t s) {
-    // a wave per candidate while the queries alone do not fill the card
-    const int threads = q.n <= 512 ? 1024 : 256;
-    hipLaunchKernelGGL(f8_finish_kernel, dim3((unsigned)q.n), dim3(threads), 0, s, v, q, ids, kp, k, D, I, id_offset, min_ord);
-    return hipGetLastError();
-}
-
-// ---- plan and launch of the first pass ----
+// ---- plans and launches ----
 static int pow2_ceil(int x) { int p = 1; while (p < x) p <<= 1; return p; }
 
 bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8SearchPlan* p) {
@@ -323,19 +570,30 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
     *p = F8SearchPlan{};
     p->kp = k + kF8Spare;
     p->r = pow2_ceil((p->kp + 63) / 64);
-    // the scan holds a register list per query and wave: eight queries of lists up to 64 keys, one of 512; its queries fit LDS
-    const int nst = (ld / kF8Block + 3) / 4;
+    const int nblk = ld / kF8Block;
+    // the scan holds a register list per query and wave (eight queries of lists up to 64 keys, one of 512) and its queries in LDS
+    const size_t per_query = (size_t)ld + 32 + (nblk + 7) / 8 * 8;
     int cap = std::max(1, 8 / p->r);
-    while (cap > 1 && (size_t)cap * (ld + 16 + nst * 4) > 128 * 1024) cap >>= 1;
+    while (cap > 1 && cap * per_query > 80 * 1024) cap >>= 1;
     p->scan = p->r <= 8 && nq <= cap;
     if (p->scan) {
         p->bt = pow2_ceil(nq);
-        p->threads = 512;
-        const size_t qb = (size_t)p->bt * (ld + 16 + nst * 4), mb = (size_t)8 * 64 * p->r * sizeof(skey_t);
-        p->lds = std::max(qb, mb);
-        const long long useful = (nrows + 127) / 128;   // eight groups of 16 rows per workgroup
-        p->grid_x = (int)std::min<long long>(num_cu, useful);
-        p->grid_y = 1;
+        p->nb = nblk == 1 || nblk == 2 || nblk == 4 ? nblk : nblk % 8 == 0 ? 8 : 0;
+        const int run_rows = p->nb ? 64 / p->nb : 8, stages = (nblk + 7) / 8;
+        const long long runs = (nrows + run_rows - 1) / run_rows;
+        // One workgroup per CU.  Whole stages keep six waves' worth of loads ahead of memory and eight only share the buffers with
+        // more (1M x 4096, one query: 611 us with six, 641 us with eight); where a wave has a handful of runs, or short
+        // stages, eight (10k x 4096: 30.0 us, with six 32.9; 2M x 768: 285 and 308).
+        const int waves = p->nb == 8 && runs >= 24ll * num_cu ? 6 : 8;
+        p->threads = waves * 64;
+        // The waves look at the candidate buffers at most p->every turns of three stages apart: no query may gain more rows
+        // meanwhile than its buffer holds beside the 63 candidates that a look may leave
+        const auto rows = [&](int turns) { return (3 * turns + stages - 1) / stages * run_rows * waves; };
+        p->cap = std::max(4096 / p->bt, rows(1) + 64);
+        for (p->every = 1; rows(2 * p->every) + 64 <= p->cap;) p->every *= 2;
+        const size_t work = std::max((size_t)p->bt * p->cap * sizeof(skey_t), p->bt > 1 ? 0 : merge_keys_bytes(waves, p->r) + (size_t)p->kp * 24);
+        p->lds = (p->bt * per_query + 15) / 16 * 16 + 64 + (size_t)p->bt * 64 * p->r * sizeof(skey_t) + work;
+        p->grid_x = (int)std::min<long long>(num_cu, (runs + waves - 1) / waves);
         p->parts = p->grid_x;
         p->kernel = "f8_scan_kernel";
     } else {
@@ -347,7 +605,6 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
         p->nslices = (int)((nrows + p->rows_per_slice - 1) / p->rows_per_slice);
         p->parts = p->nslices;
         p->grid_x = p->nqt * p->nslices;
-        p->grid_y = 1;
         p->threads = 512;
         p->lds = (size_t)2 * (256 + p->tq) * 128 + EPI_LDS_BYTES;
         p->cand_bytes = (size_t)p->grid_x * 256 * CAND_CAP * sizeof(skey_t);
@@ -358,15 +615,61 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
     return true;
 }
 
-template <int BT, int R>
-static hipError_t launch_scan(const F8View& v, const F8Mat& q, const F8SearchPlan& p, skey_t* partial, const TailMerge& tail, hipStream_t s) {
+template <int BT, int R, int NB>
+static hipError_t launch_scan_nb(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s) {
     if (p.lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_scan_kernel<BT, R>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_scan_kernel<BT, R, NB>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((f8_scan_kernel<BT, R>), dim3(p.grid_x, p.grid_y), dim3(p.threads), p.lds, s, v, q, p.kp, partial, tail);
+    hipLaunchKernelGGL((f8_scan_kernel<BT, R, NB>), dim3(p.grid_x), dim3(p.threads), p.lds, s, a);
     return hipGetLastError();
 }
+template <int BT, int R>
+static hipError_t launch_scan(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s) {
+    if (p.nb == 1) return launch_scan_nb<BT, R, 1>(a, p, s);
+    if (p.nb == 2) return launch_scan_nb<BT, R, 2>(a, p, s);
+    if (p.nb == 4) return launch_scan_nb<BT, R, 4>(a, p, s);
+    if (p.nb == 8) return launch_scan_nb<BT, R, 8>(a, p, s);
+    return launch_scan_nb<BT, R, 0>(a, p, s);
+}
+template <int R>
+static hipError_t launch_finish_r(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s) {
+    const int threads = R == 16 ? 256 : 512;   // (the lists of the waves meet in LDS)
+    const int ld = a.v.X.ld;
+    const size_t lds = (size_t)(ld + ld / kF8Block + 15) / 16 * 16 + merge_keys_bytes(threads / 64, R) + (size_t)p.kp * 24;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_finish_kernel<R>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(f8_finish_kernel<R>, dim3((unsigned)a.q.n), dim3(threads), lds, s, a, p.parts);
+    return hipGetLastError();
+}
+hipError_t launch_f8_finish(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s) {
+    switch (p.r) {
+        case 1: return launch_finish_r<1>(a, p, s);
+        case 2: return launch_finish_r<2>(a, p, s);
+        case 4: return launch_finish_r<4>(a, p, s);
+        case 8: return launch_finish_r<8>(a, p, s);
+        case 16: return launch_finish_r<16>(a, p, s);
+    }
+    return hipErrorInvalidValue;
+}
+hipError_t launch_f8_scan(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s) {
+    switch (p.r * 16 + p.bt) {
+        case 16 + 1: return launch_scan<1, 1>(a, p, s);
+        case 16 + 2: return launch_scan<2, 1>(a, p, s);
+        case 16 + 4: return launch_scan<4, 1>(a, p, s);
+        case 16 + 8: return launch_scan<8, 1>(a, p, s);
+        case 32 + 1: return launch_scan<1, 2>(a, p, s);
+        case 32 + 2: return launch_scan<2, 2>(a, p, s);
+        case 32 + 4: return launch_scan<4, 2>(a, p, s);
+        case 64 + 1: return launch_scan<1, 4>(a, p, s);
+        case 64 + 2: return launch_scan<2, 4>(a, p, s);
+        case 128 + 1: return launch_scan<1, 8>(a, p, s);
+    }
+    return hipErrorInvalidValue;
+}
+
 template <int MT, int NT, int WM, int WN, int R>
 static hipError_t launch_tile(const F8View& v, const F8Mat& q, const F8SearchPlan& p, const MfmaParams& P, hipStream_t s) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_search_tile_kernel<MT, NT, WM, WN, R>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
@@ -375,17 +678,11 @@ static hipError_t launch_tile(const F8View& v, const F8Mat& q, const F8SearchPla
     return hipGetLastError();
 }
 template <int R>
-static hipError_t launch_r(const F8View& v, const F8Mat& q, const F8SearchPlan& p, void* share, void* cand, skey_t* partial, const TailMerge& tail, hipStream_t s) {
-    if (p.scan) {
-        if constexpr (R == 1) {
-            if (p.bt == 8) return launch_scan<8, 1>(v, q, p, partial, tail, s);
-            if (p.bt == 4) return launch_scan<4, 1>(v, q, p, partial, tail, s);
-        }
-        if constexpr (R == 2) { if (p.bt == 4) return launch_scan<4, 2>(v, q, p, partial, tail, s); }
-        if constexpr (R <= 4) { if (p.bt == 2) return launch_scan<2, R>(v, q, p, partial, tail, s); }
-        if constexpr (R <= 8) { if (p.bt == 1) return launch_scan<1, R>(v, q, p, partial, tail, s); }
-        return hipErrorInvalidValue;
-    }
+static hipError_t launch_r(const F8View& v, const F8Mat& q, const F8SearchPlan& p, const MfmaParams& P, hipStream_t s) {
+    if (p.tq == 64) return launch_tile<2, 4, 8, 1, R>(v, q, p, P, s);
+    return launch_tile<4, 4, 4, 2, R>(v, q, p, P, s);
+}
+hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& p, void* share, void* cand, skey_t* partial, hipStream_t s) {
     MfmaParams P = {};
     P.nq = (int)q.n;
     P.k = p.kp;
@@ -398,18 +695,12 @@ static hipError_t launch_r(const F8View& v, const F8Mat& q, const F8SearchPlan& 
     P.gthr = static_cast<unsigned*>(share);
     const int words = p.nqt * p.tq;
     hipLaunchKernelGGL(f8_zero_kernel, dim3((words + 255) / 256), dim3(256), 0, s, P.gthr, words);
-    if (p.tq == 64) return launch_tile<2, 4, 8, 1, R>(v, q, p, P, s);
-    return launch_tile<4, 4, 4, 2, R>(v, q, p, P, s);
-}
-hipError_t launch_f8_search(const F8View& v, const F8Mat& q, int k, const F8SearchPlan& p, void* share, void* cand, skey_t* partial,
-                            const TailMerge& tail, hipStream_t s) {
-    (void)k;
     switch (p.r) {
-        case 1: return launch_r<1>(v, q, p, share, cand, partial, tail, s);
-        case 2: return launch_r<2>(v, q, p, share, cand, partial, tail, s);
-        case 4: return launch_r<4>(v, q, p, share, cand, partial, tail, s);
-        case 8: return launch_r<8>(v, q, p, share, cand, partial, tail, s);
-        case 16: return launch_r<16>(v, q, p, share, cand, partial, tail, s);
+        case 1: return launch_r<1>(v, q, p, P, s);
+        case 2: return launch_r<2>(v, q, p, P, s);
+        case 4: return launch_r<4>(v, q, p, P, s);
+        case 8: return launch_r<8>(v, q, p, P, s);
+        case 16: return launch_r<16>(v, q, p, P, s);
     }
     return hipErrorInvalidValue;
 }

@@ -22,8 +22,8 @@ def _blocks(d: int) -> int:
     return (d + BLOCK - 1) // BLOCK
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# handle of the current torch stream of device i (the Stream object around it costs more than a launch)
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _rows_arg(x, what: str) -> torch.Tensor:
@@ -46,15 +46,41 @@ def _stride(x: torch.Tensor) -> int:
 class F8Rows:
     """n rows of d elements in 8 bits: `codes` (n, whole blocks of 128) float8_e4m3fn, `scales` (n, >= blocks) uint8."""
 
+    __slots__ = ("n", "d", "device_index", "_args", "_buffer", "_codes", "_scales")
+
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, d: int):
-        self.codes, self.scales, self.d = codes, scales, int(d)
+        self.n, self.d, self._codes, self._scales, self._buffer = codes.shape[0], int(d), codes, scales, None
+        self.device_index = codes.get_device()
+        # codes, their stride, scales, their stride: as the C entry points take them
+        self._args = (codes.data_ptr(), codes.stride(0) if self.n > 1 else codes.shape[1],
+                      scales.data_ptr(), scales.stride(0) if self.n > 1 else (scales.shape[1] + 3) // 4 * 4)
 
     @classmethod
     def empty(cls, n: int, d: int, device) -> "F8Rows":
-        """Rows to be written by quantize_f8 / rms_norm_f8 (`out=`)."""
+        """Rows to be written by quantize_f8 / rms_norm_f8 (`out=`): one allocation, the codes and behind them the scales."""
         blocks = _blocks(d)
-        return cls(torch.empty((n, blocks * BLOCK), dtype=torch.float8_e4m3fn, device=device),
-                   torch.empty((n, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=device), d)
+        ld, ls = blocks * BLOCK, (blocks + 3) // 4 * 4
+        self = cls.__new__(cls)
+        self.n, self.d, self._codes, self._scales = n, d, None, None
+        self._buffer = buf = torch.empty(n * (ld + ls), dtype=torch.uint8, device=device)
+        self.device_index = buf.get_device()
+        p = buf.data_ptr()
+        self._args = (p, ld, p + n * ld, ls)
+        return self
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            ld = _blocks(self.d) * BLOCK
+            self._codes = self._buffer[:self.n * ld].view(self.n, ld).view(torch.float8_e4m3fn)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            blocks = _blocks(self.d)
+            self._scales = self._buffer[self.n * blocks * BLOCK:].view(self.n, (blocks + 3) // 4 * 4)
+        return self._scales
 
     @classmethod
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, d: Optional[int] = None) -> "F8Rows":
@@ -84,12 +110,8 @@ class F8Rows:
         return cls(raw.view(torch.float8_e4m3fn), scales, d)
 
     @property
-    def n(self) -> int:
-        return self.codes.shape[0]
-
-    @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return torch.device("cuda", self.device_index)
 
     def __len__(self) -> int:
         return self.n
@@ -100,25 +122,21 @@ class F8Rows:
             raise TypeError("F8Rows: only plain slices of rows")
         return F8Rows(self.codes[rows], self.scales[rows], self.d)
 
-    def _abi(self):
-        """(codes, stride, scales, stride) as the C entry points take them."""
-        c, s = self.codes, self.scales
-        return (c.data_ptr(), c.stride(0) if self.n > 1 else c.shape[1], s.data_ptr(), s.stride(0) if self.n > 1 else (s.shape[1] + 3) // 4 * 4)
-
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the rows stand for, (n, d); exact in float32 and bfloat16 (four significant bits times a power of two)."""
         if dtype not in _SRC:
             raise TypeError(f"dequantize: expected float32, float16 or bfloat16, got {dtype}")
-        out = torch.empty((self.n, self.d), dtype=dtype, device=self.device)
-        _lib.check(_lib.load().ssmi_f8_dequantize(self.device.index, self.n, self.d, *self._abi(), out.data_ptr(), _SRC[dtype], self.d, _stream(self.device)))
+        i = self.device_index
+        out = torch.empty((self.n, self.d), dtype=dtype, device=i)
+        _lib.check(_lib.load().ssmi_f8_dequantize(i, self.n, self.d, *self._args, out.data_ptr(), _SRC[dtype], self.d, _stream(i)))
         return out
 
 
-def _out_rows(out: Optional[F8Rows], n: int, d: int, device: torch.device, what: str) -> F8Rows:
+def _out_rows(out: Optional[F8Rows], n: int, d: int, device_index: int, what: str) -> F8Rows:
     if out is None:
-        return F8Rows.empty(n, d, device)
-    if not isinstance(out, F8Rows) or out.n != n or out.d != d or out.device != device:
-        raise ValueError(f"{what}: out must be F8Rows of {n} rows of {d} elements on {device}")
+        return F8Rows.empty(n, d, device_index)
+    if not isinstance(out, F8Rows) or out.n != n or out.d != d or out.device_index != device_index:
+        raise ValueError(f"{what}: out must be F8Rows of {n} rows of {d} elements on cuda:{device_index}")
     return out
 
 
@@ -126,19 +144,21 @@ def quantize_f8(x: torch.Tensor, out: Optional[F8Rows] = None) -> F8Rows:
     """8-bit rows of x (n, d): per 128 elements the smallest power of two s with max|x| <= 448 s, codes x / s to nearest even."""
     x = _rows_arg(x, "quantize_f8")
     n, d = x.shape
-    out = _out_rows(out, n, d, x.device, "quantize_f8")
-    _lib.check(_lib.load().ssmi_f8_quantize(x.device.index, n, d, x.data_ptr(), _SRC[x.dtype], _stride(x), *out._abi(), _stream(x.device)))
+    i = x.get_device()
+    out = _out_rows(out, n, d, i, "quantize_f8")
+    _lib.check(_lib.load().ssmi_f8_quantize(i, n, d, x.data_ptr(), _SRC[x.dtype], _stride(x), *out._args, _stream(i)))
     return out
 
 
 def rms_norm_f8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                 residual_out: Optional[torch.Tensor] = None, eps: float = 1e-6, unit: bool = False, out: Optional[F8Rows] = None) -> F8Rows:
-    """8-bit rows of the root-mean-square norm of h = x + residual: h / sqrt(mean(h^2) + eps) * weight, sums in float32.
+    """8-bit rows of the root-mean-square norm of h = x + residual: h / sqrt(mean(h^2) + eps) * weight, in 64 bits.
 
     The sum is rounded to x's type and stored in `residual_out` (default: back into `residual`).  unit=True: rows of unit length,
     ready for an inner-product index."""
     x = _rows_arg(x, "rms_norm_f8")
     n, d = x.shape
+    i = x.get_device()
     w = r = ro = None
     if weight is not None:
         if not isinstance(weight, torch.Tensor) or weight.shape != (d,) or weight.device != x.device:
@@ -158,11 +178,11 @@ def rms_norm_f8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual
             r = r.contiguous()
     elif residual_out is not None:
         raise ValueError("rms_norm_f8: residual_out without a residual")
-    out = _out_rows(out, n, d, x.device, "rms_norm_f8")
+    out = _out_rows(out, n, d, i, "rms_norm_f8")
     _lib.check(_lib.load().ssmi_f8_rms_norm(
-        x.device.index, n, d, x.data_ptr(), _SRC[x.dtype], _stride(x), r.data_ptr() if r is not None else None, _stride(r) if r is not None else 0,
+        i, n, d, x.data_ptr(), _SRC[x.dtype], _stride(x), r.data_ptr() if r is not None else None, _stride(r) if r is not None else 0,
         ro.data_ptr() if ro is not None else None, _stride(ro) if ro is not None else 0, w.data_ptr() if w is not None else None,
-        _SRC[w.dtype] if w is not None else 0, float(eps), 1 if unit else 0, *out._abi(), _stream(x.device)))
+        _SRC[w.dtype] if w is not None else 0, float(eps), 1 if unit else 0, *out._args, _stream(i)))
     return out
 
 
@@ -172,16 +192,17 @@ def matmul_f8(a: F8Rows, b: F8Rows, out_dtype: torch.dtype = torch.bfloat16, out
         raise TypeError("matmul_f8: expected two F8Rows")
     if a.d != b.d:
         raise ValueError(f"matmul_f8: rows of {a.d} and {b.d} elements")
-    if a.device != b.device:
+    i = a.device_index
+    if i != b.device_index:
         raise ValueError(f"matmul_f8: operands on {a.device} and {b.device}")
     if out is not None:
         out_dtype = out.dtype
     if out_dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"matmul_f8: the output is float16 or bfloat16, not {out_dtype}")
     if out is None:
-        out = torch.empty((a.n, b.n), dtype=out_dtype, device=a.device)
-    elif out.shape != (a.n, b.n) or out.device != a.device or (b.n > 1 and out.stride(1) != 1) or (a.n > 1 and out.stride(0) < b.n):
+        out = torch.empty((a.n, b.n), dtype=out_dtype, device=i)
+    elif out.shape != (a.n, b.n) or out.get_device() != i or (b.n > 1 and out.stride(1) != 1) or (a.n > 1 and out.stride(0) < b.n):
         raise ValueError(f"matmul_f8: out must be ({a.n}, {b.n}) with contiguous rows on {a.device}")
-    _lib.check(_lib.load().ssmi_f8_matmul(a.device.index, a.n, b.n, a.d, *a._abi(), *b._abi(), out.data_ptr(), _SRC[out_dtype],
-                                          out.stride(0) if a.n > 1 else b.n, _stream(a.device)))
+    _lib.check(_lib.load().ssmi_f8_matmul(i, a.n, b.n, a.d, *a._args, *b._args, out.data_ptr(), _SRC[out_dtype],
+                                          out.stride(0) if a.n > 1 else b.n, _stream(i)))
     return out

@@ -166,7 +166,7 @@ class _IndexBase:
 
     def _check_f8(self, x: F8Rows, what: str) -> None:
         assert x.d == self.d, f"{what}: dimension {x.d} != index dimension {self.d}"
-        if x.device.index != self.device:
+        if x.device_index != self.device:
             raise RuntimeError(f"{what}: rows are on {x.device}, index lives on cuda:{self.device}")
 
     def _device_out(self, out, nq: int, k: int, device):
@@ -184,7 +184,7 @@ class _IndexBase:
         if isinstance(x, F8Rows):
             self._check_f8(x, "add")
             torch.cuda.current_stream(x.device).synchronize()  # the library copies on its own stream
-            _lib.check(self._lib.ssmi_index_add_f8(self._handle(), x.n, *x._abi()))
+            _lib.check(self._lib.ssmi_index_add_f8(self._handle(), x.n, *x._args))
             return
         if isinstance(x, torch.Tensor) and x.is_cuda:
             self._check_tensor(x, "add")
@@ -220,7 +220,7 @@ class _IndexBase:
             self._check_f8(x, "search")
             D, I = self._device_out(out, x.n, k, x.device)
             stream = torch.cuda.current_stream(x.device).cuda_stream
-            _lib.check(self._lib.ssmi_index_search_f8(self._handle(), x.n, *x._abi(), k, floor, D.data_ptr(), I.data_ptr(),
+            _lib.check(self._lib.ssmi_index_search_f8(self._handle(), x.n, *x._args, k, floor, D.data_ptr(), I.data_ptr(),
                                                       int(id_offset), stream))
             return D, I
         if isinstance(x, torch.Tensor) and x.is_cuda:
