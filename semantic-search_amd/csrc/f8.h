@@ -18,7 +18,7 @@ namespace ssmi {
 static constexpr int kF8 = 3;             // SSMI_F8
 static constexpr int kF8Block = 128;      // codes per scale
 static constexpr int kF8Spare = 16;       // candidates beyond k that a search scores again in 64 bits
-static constexpr int kF8MaxNorm = 32768;  // elements of a row that the norm keeps in registers
+static constexpr int kF8MaxNorm = 16384;  // elements of a row that the norm keeps in registers
 static constexpr int kF8MaxK = kMaxK - kF8Spare;
 
 inline int f8_ld(int d) { return (d + kF8Block - 1) / kF8Block * kF8Block; }

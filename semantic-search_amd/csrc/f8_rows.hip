@@ -74,7 +74,7 @@ __device__ __forceinline__ void row_sums(double& a, double& b, double2* lds) {
 // The norm's sums and its one factor per row are 64-bit: y is then the exact value rounded once, and an element's code is that of
 // the exact row unless y lies within 2^-24 of a border.  (With fp32 sums and factors three times as many codes parted from the exact
 // ones; the 64-bit products hide behind memory.)  unit needs no second pass: |y| = f |h w| for y = f h w.
-// (Eight passes of 1024 threads would take rows of 65536 elements through the norm too, but spill.)
+// (Four passes of 1024 threads would take rows of 32768 elements through the norm, but spill.)
 template <typename T, int ITER, bool WAVE, bool VEC, bool NORM>
 __global__ void __launch_bounds__(WAVE ? 256 : 1024) f8_rows_kernel(F8NormArgs a) {
     __shared__ double2 red[16];
@@ -172,10 +172,10 @@ static hipError_t launch_rows_t(const F8NormArgs& a, int num_cu, hipStream_t s) 
     } else {
         threads = per <= 64 ? 64 : per <= 128 ? 128 : per <= 256 ? 256 : per <= 512 ? 512 : 1024;
         // many rows: half the threads and two passes of a row each keep more rows in flight per CU
-        if (a.n >= 4ll * num_cu && threads >= 512) threads = per <= 2048 ? 256 : 1024;
+        if (a.n >= 4ll * num_cu && threads >= 512) threads = per <= 512 ? 256 : per <= 1024 ? 512 : 1024;
         iter = (per + threads - 1) / threads;
     }
-    iter = iter <= 1 ? 1 : iter <= 2 ? 2 : 4;
+    iter = iter <= 1 ? 1 : iter <= 2 || !wave ? 2 : 4;
     const long long blocks = wave ? (a.n + 3) / 4 : a.n;
     const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
 #define GO(I, W, V) { if (a.norm) hipLaunchKernelGGL((f8_rows_kernel<T, I, W, V, true>), grid, dim3(threads), 0, s, a); \
@@ -183,8 +183,7 @@ static hipError_t launch_rows_t(const F8NormArgs& a, int num_cu, hipStream_t s) 
 #define GO_V(I, W) { if (vec) GO(I, W, true) else GO(I, W, false) }
     if (wave) { if (iter == 1) GO_V(1, true) else if (iter == 2) GO_V(2, true) else GO_V(4, true) }
     else if (iter == 1) GO_V(1, false)
-    else if (iter == 2) GO_V(2, false)
-    else GO_V(4, false)
+    else GO_V(2, false)
 #undef GO_V
 #undef GO
     return hipGetLastError();
