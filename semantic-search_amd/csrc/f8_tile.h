@@ -25,6 +25,13 @@ __device__ __forceinline__ i32x8_t join8(const i32x4_t& lo, const i32x4_t& hi) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+template <int J>
+__device__ __forceinline__ f32x16_t mfma_f8_32(const i32x8_t& a, const i32x8_t& b, const f32x16_t& c, int sa, int sb) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, J, sa, J, sb);
+}
+
 // One operand's tile: rows of a plain matrix or of one segment of a row store (uniform base, 32-bit offsets).
 struct F8Src {
     const unsigned char* codes;   // row 0 of the tile
