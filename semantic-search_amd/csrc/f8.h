@@ -69,7 +69,7 @@ struct F8SearchPlan {
     int bt, r, threads, grid_x;
     int nb;                   // scan: blocks per row where that is 1, 2 or 4, 8 where it is a multiple of 8, else 0
     int cap, every;           // scan: candidates a query's buffer holds, turns of three stages between two looks at them
-    int tq, nqt, nslices;
+    int tq, nqt, nslices, gtop_m;
     long long rows_per_slice;
     size_t lds, partial_bytes, cand_bytes, share_bytes;
     const char* kernel;

@@ -7,7 +7,7 @@
 // 2^-53 - and sorts them by that, ties by the lower id.  A query therefore gets the same ids and scores in any batch.
 //
 // Same place on the path as the 16-bit kernels: faiss.IndexFlatIP.search as called from core/index_manager.py:371.
-#include "f8_tile.h"
+#include "f8_pp.h"
 #include "tail_merge.h"
 #include <algorithm>
 
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, 
         __syncthreads();
         ++tiles_done;
         // fold after row tiles 1, 4, 16, ... of the slice and whenever a candidate buffer is half full
-        if (((tiles_done & (tiles_done - 1)) == 0 && (tiles_done & 0x55555555u)) || *flag_l) {
+        if (((tiles_done & (tiles_done - 1)) == 0 && (tiles_done & P.fold_mask)) || *flag_l) {
             fold_queries<R>(wave, q0, P, slice, cand, thr_l, cnt_l, kept_l);
             if (lane < 32) {   // the k-th score of any slice bounds the final one: the slices share the highest (mfma.hip)
                 const int ql = wave + 8 * lane;
@@ -557,9 +557,170 @@ __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, 
     fold_queries<R>(wave, q0, P, slice, cand, thr_l, cnt_l, kept_l);
 }
 
-__global__ void f8_zero_kernel(unsigned* p, int n) {
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < n) p[i] = 0;
+// ---- large batches: 256 rows x 256 queries on the contraction of f8_pp.h ----
+// Threshold filter over a wave's 128 x 64 accumulators (acc[m][n][4 g + e]: row row_base + 32 m + 8 g + 4 h + e, query q_base + 32 n + r
+// of lane (r, h)): as filter_tile of the 16-bit kernels, one column maximum first, survivors one by one.
+// seed: first row tile of a slice, whole, and kp <= 64: no list exists yet and every row would pass.  The lane's 64 rows
+// of a query are taken in pairs and the 32 maxima sorted; at least c = ceil(kp / 2) rows of each of the two lanes of a column reach the
+// lane's c-th, so the smaller of the two has kp of this wave's rows at or above it and may serve as threshold for this tile.
+template <bool FULL>
+__device__ __forceinline__ void filter_big(const F8Pp::Acc& acc, int row_base, int q_base, int lane, long long row0, int rows_valid, skey_t* cand,
+                                           const float* thr_l, unsigned* cnt_l, unsigned* flag_l, int seed) {
+    const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int ql = q_base + 32 * n + r;
+        float thr = thr_l[ql];
+        if (FULL && seed) {
+            float v[32];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const f32x16_t a = acc[m][n];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[m * 8 + i] = vmax3(a[2 * i], a[2 * i + 1], SSMI_NEG_MAX);   // (no NaN may enter the sort: it would double its partner)
+            }
+#pragma unroll
+            for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+                for (int st = size >> 1; st >= 1; st >>= 1)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if ((i & st) == 0) {
+                            const float a = v[i], b = v[i + st];
+                            const bool desc = (i & size) == 0 || size == 32;
+                            v[i] = desc ? fmaxf(a, b) : fminf(a, b);
+                            v[i + st] = desc ? fminf(a, b) : fmaxf(a, b);
+                        }
+            float t = v[0];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) t = i < seed ? v[i] : t;
+            thr = fmaxf(thr, fminf(t, __int_as_float(xor_lane<32>(__float_as_int(t)))));
+        }
+        float mm[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const f32x16_t v = acc[m][n];
+            float a = vmax3(v[0], v[1], v[2]);
+#pragma unroll
+            for (int i = 3; i < 15; i += 2) a = vmax3(a, v[i], v[i + 1]);
+            mm[m] = vmax2(a, v[15]);
+        }
+        const float mx = vmax2(vmax3(mm[0], mm[1], mm[2]), mm[3]);
+        if (__builtin_amdgcn_ballot_w64(mx >= thr) == 0) continue;
+        if (mx >= thr) {
+            skey_t* cq = cand + (size_t)ql * CAND_CAP;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(mm[m] >= thr) != 0, 0)) {
+                    const f32x16_t v = acc[m][n];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float s = v[i];
+                        const int rr = row_base + 32 * m + 8 * (i >> 2) + 4 * h + (i & 3);
+                        if (s >= thr && (FULL || rr < rows_valid)) {
+                            const unsigned pos = lds_add_rtn(&cnt_l[ql], 1u);
+                            if (pos + 1 >= (unsigned)CAND_TRIG) lds_store(flag_l, 1u);
+                            if (pos < (unsigned)CAND_CAP) cq[pos] = make_key(s, (uint32_t)(row0 + rr));
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+// A workgroup keeps its query tile and walks a slice of the rows; the first slab of the next row tile travels under this one's filter.
+// Folds, thresholds and the bound from the slices' published tops are those of the 16-bit kernel (mfma_pp.hip).
+template <int R>
+__global__ void __launch_bounds__(512, 2) f8_search_big_kernel(F8View V, F8Mat q, MfmaParams P) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    float* thr_l = reinterpret_cast<float*>(smem + F8Pp::LDS);
+    unsigned* cnt_l = reinterpret_cast<unsigned*>(thr_l + 256);
+    unsigned* kept_l = cnt_l + 256;
+    unsigned* flag_l = kept_l + 256;
+    F8Pp t;
+    t.init(smem, V.X.ld / kF8Block);
+    int logical = blockIdx.x;
+    if ((gridDim.x & 7) == 0) logical = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const int slice = logical / P.nqt, qt = logical % P.nqt;
+    const int q0 = qt * 256;
+    const long long r_begin = (long long)slice * P.rows_per_slice;
+    const long long r_end = min(r_begin + P.rows_per_slice, V.X.nrows);
+    skey_t* cand = P.cand + (size_t)blockIdx.x * 256 * CAND_CAP;
+    if (threadIdx.x < 256) {
+        thr_l[threadIdx.x] = q0 + (int)threadIdx.x < P.nq ? P.thr_floor : __builtin_inff();
+        cnt_l[threadIdx.x] = 0;
+        kept_l[threadIdx.x] = 0;
+    }
+    if (threadIdx.x == 0) flag_l[0] = 0;
+    __syncthreads();
+    const long long seg_mask = (1ll << V.X.seg_shift) - 1;
+    const F8Src qsrc{q.codes + (size_t)q0 * q.stride, q.scales + (size_t)q0 * q.sstride, (unsigned)q.stride, (unsigned)q.sstride, (int)min(255ll, q.n - 1 - q0)};
+    auto aim = [&](long long row0) __attribute__((always_inline)) {
+        const long long seg = row0 >> V.X.seg_shift, off = row0 & seg_mask;
+        t.aim(F8Src{static_cast<const unsigned char*>(V.X.segs[seg]) + off * V.X.ld, static_cast<const unsigned char*>(V.ssegs[seg]) + off * V.sld,
+                    (unsigned)V.X.ld, (unsigned)V.sld, (int)min(255ll, r_end - 1 - row0)}, qsrc);
+    };
+    auto push_bounds = [&](int lane) {
+        for (int ql = slice + t.wave * P.nslices; ql < 256 && q0 + ql < P.nq; ql += 8 * P.nslices) {
+            const unsigned b = tops_bound(P, q0 + ql);
+            if (b && lane == 0) atomicMax(&P.gthr[q0 + ql], b);
+        }
+    };
+    auto pull_thr = [&](int lane) {
+        const int ql = t.wave + 8 * lane;
+        if (lane < 32 && q0 + ql < P.nq) {
+            const unsigned seen = __hip_atomic_load(&P.gthr[q0 + ql], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (seen && ord_to_f32(seen) > thr_l[ql]) lds_store(reinterpret_cast<unsigned*>(&thr_l[ql]), __float_as_uint(ord_to_f32(seen)));
+        }
+    };
+    const int seed_c = P.k <= 64 ? (P.k + 1) / 2 : 0;
+    unsigned tiles_done = 0;
+    int xstate = 0;
+    if (r_begin < r_end) aim(r_begin);
+#pragma unroll 1
+    for (long long row0 = r_begin; row0 < r_end; row0 += 256) {
+        F8Pp::Acc acc;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
+        t.run(acc);
+        const long long left = r_end - row0;
+        if (row0 + 256 < r_end) aim(row0 + 256);
+        const int lane = t.lane;
+        if (left >= 256) filter_big<true>(acc, t.wm * 128, t.wn * 64, lane, row0, 256, cand, thr_l, cnt_l, flag_l, tiles_done == 0 ? seed_c : 0);
+        else filter_big<false>(acc, t.wm * 128, t.wn * 64, lane, row0, (int)left, cand, thr_l, cnt_l, flag_l, 0);
+        __syncthreads();
+        ++tiles_done;
+        const bool fold_due = ((tiles_done & (tiles_done - 1)) == 0 && (tiles_done & P.fold_mask)) || *flag_l;
+        if (xstate && !fold_due) {
+            if (xstate == 1) push_bounds(lane); else pull_thr(lane);
+            xstate = xstate == 1 ? 2 : 0;
+        }
+        if (fold_due) {
+            fold_queries<R>(t.wave, q0, P, slice, cand, thr_l, cnt_l, kept_l);
+            xstate = P.gtop ? 1 : 0;
+            __syncthreads();
+            const int ql = t.wave + 8 * lane;
+            if (lane < 32 && q0 + ql < P.nq) {
+                const float th = thr_l[ql];
+                const unsigned mine = th > SSMI_NEG_MAX ? f32_to_ord(th) : 0u;
+                const unsigned seen = atomicMax(&P.gthr[q0 + ql], mine);
+                if (seen > mine) thr_l[ql] = ord_to_f32(seen);
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) *flag_l = 0;
+        }
+    }
+    __syncthreads();
+    fold_queries<R>(t.wave, q0, P, slice, cand, thr_l, cnt_l, kept_l);
+}
+
+__global__ void f8_zero_kernel(unsigned* p, size_t n) {
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) p[i] = 0;
 }
 
 // ---- plans and launches ----
@@ -597,7 +758,7 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
         p->parts = p->grid_x;
         p->kernel = "f8_scan_kernel";
     } else {
-        p->tq = nq <= 64 ? 64 : 128;
+        p->tq = nq <= 64 ? 64 : nq <= 128 ? 128 : 256;
         p->nqt = (nq + p->tq - 1) / p->tq;
         const long long tiles = (nrows + 255) / 256;
         const long long ns = std::max<long long>(1, std::min<long long>(num_cu / p->nqt, tiles));
@@ -606,10 +767,14 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
         p->parts = p->nslices;
         p->grid_x = p->nqt * p->nslices;
         p->threads = 512;
-        p->lds = (size_t)2 * (256 + p->tq) * 128 + EPI_LDS_BYTES;
+        p->lds = (p->tq == 256 ? (size_t)F8Pp::LDS : (size_t)2 * (256 + p->tq) * 128) + EPI_LDS_BYTES;
         p->cand_bytes = (size_t)p->grid_x * 256 * CAND_CAP * sizeof(skey_t);
-        p->share_bytes = (size_t)p->nqt * p->tq * sizeof(unsigned);
-        p->kernel = "f8_search_tile_kernel";
+        // scores every slice publishes per query: enough that the kp-th largest of all of them exists and is tight (mfma.hip)
+        int m = (int)((std::max<long long>(64, (long long)p->kp * 5 / 4) + p->nslices - 1) / p->nslices);
+        m = std::max(1, std::min(std::min(m, 8), p->kp));
+        p->gtop_m = (p->tq == 256 && p->nslices > 1 && (long long)p->nslices * m >= p->kp) ? m : 0;
+        p->share_bytes = (size_t)p->nqt * p->tq * (1 + (size_t)p->nslices * p->gtop_m) * sizeof(unsigned);
+        p->kernel = p->tq == 256 ? "f8_search_big_kernel" : "f8_search_tile_kernel";
     }
     p->partial_bytes = (size_t)nq * p->parts * p->kp * sizeof(skey_t);
     return true;
@@ -680,7 +845,11 @@ static hipError_t launch_tile(const F8View& v, const F8Mat& q, const F8SearchPla
 template <int R>
 static hipError_t launch_r(const F8View& v, const F8Mat& q, const F8SearchPlan& p, const MfmaParams& P, hipStream_t s) {
     if (p.tq == 64) return launch_tile<2, 4, 8, 1, R>(v, q, p, P, s);
-    return launch_tile<4, 4, 4, 2, R>(v, q, p, P, s);
+    if (p.tq == 128) return launch_tile<4, 4, 4, 2, R>(v, q, p, P, s);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_search_big_kernel<R>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(f8_search_big_kernel<R>, dim3(p.grid_x), dim3(p.threads), p.lds, s, v, q, P);
+    return hipGetLastError();
 }
 hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& p, void* share, void* cand, skey_t* partial, hipStream_t s) {
     MfmaParams P = {};
@@ -693,8 +862,11 @@ hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& 
     P.cand = static_cast<skey_t*>(cand);
     P.thr_floor = SSMI_NEG_MAX;
     P.gthr = static_cast<unsigned*>(share);
-    const int words = p.nqt * p.tq;
-    hipLaunchKernelGGL(f8_zero_kernel, dim3((words + 255) / 256), dim3(256), 0, s, P.gthr, words);
+    P.gtop = p.gtop_m ? P.gthr + (size_t)p.nqt * p.tq : nullptr;
+    P.gtop_m = p.gtop_m;
+    P.fold_mask = P.gtop ? 0x11111111u : 0x55555555u;   // scheduled folds after row tiles 1, 16, 256, ... (1, 4, 16, ... without the bound)
+    const size_t words = p.share_bytes / sizeof(unsigned);
+    hipLaunchKernelGGL(f8_zero_kernel, dim3((unsigned)std::min<size_t>((words + 255) / 256, 4096)), dim3(256), 0, s, P.gthr, words);
     switch (p.r) {
         case 1: return launch_r<1>(v, q, p, P, s);
         case 2: return launch_r<2>(v, q, p, P, s);
