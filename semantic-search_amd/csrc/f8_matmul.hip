@@ -2,8 +2,10 @@
 //
 //   out[i][j] = sum over blocks b of 2^(sa[i,b] - 127) 2^(sb[j,b] - 127) sum over the 128 codes of b of a[i,.] b[j,.]
 //
-// rounded once to 16 bits.  Tiles of 256 x 256 where there are enough of them for every CU, tiles of 128 x 128 below that, and for a
-// few rows of `a` (a decoding batch) a kernel that streams the rows of `b` straight into registers, bound by reading `b` once.
+// rounded once to 16 bits.  Tiles of 256 x 256 with a wave per SIMD where they fill the chip, tiles of 128 x 128 and 64 x 64 below
+// that, and where those would leave most CUs idle (a decoding batch) smaller ones whose waves share K.
+#include <algorithm>
+#include <initializer_list>
 #include "f8_big.h"
 
 namespace ssmi {
@@ -27,7 +29,6 @@ struct F8MatmulArgs {
     int nblk;
     unsigned short* out;
     long long ostride;
-    bool vec, vec8; // four (eight) neighbours leave as one 8-byte (16-byte) store
     int ta, tb;     // tiles along a and b
 };
 
@@ -36,19 +37,22 @@ struct F8Out {
     unsigned short* base;
     long long ostride;
     int rows, cols;
-    bool vec, vec8;
 };
 __device__ __forceinline__ F8Out out_tile(const F8MatmulArgs& p, long long i0, long long j0) {
-    return F8Out{p.out + i0 * p.ostride + j0, p.ostride, (int)min(256ll, p.a.n - i0), (int)min(256ll, p.b.n - j0), p.vec, p.vec8};
+    return F8Out{p.out + i0 * p.ostride + j0, p.ostride, (int)min(256ll, p.a.n - i0), (int)min(256ll, p.b.n - j0)};
 }
-// N neighbouring columns c.. of row r, two to a word
+// N neighbouring columns c.. of row r, two to a word, as one store: the memory takes 8 and 16 bytes at any even address, and rows
+// of an odd stride need no other path
 template <int N>
-__device__ __forceinline__ void store_words(const F8Out& t, bool vec, int r, int c, const unsigned (&w)[N / 2]) {
+__device__ __forceinline__ void store_words(const F8Out& t, int r, int c, const unsigned (&w)[N / 2]) {
+    typedef unsigned words_t __attribute__((ext_vector_type(N / 2), aligned(2)));
     if (r >= t.rows || c >= t.cols) return;
     unsigned short* o = t.base + (unsigned long long)(unsigned)r * (unsigned long long)t.ostride + c;
-    if (vec && c + N <= t.cols) {
-        if constexpr (N == 8) *reinterpret_cast<uint4*>(o) = uint4{w[0], w[1], w[2], w[3]};
-        else *reinterpret_cast<uint2*>(o) = uint2{w[0], w[1]};
+    if (c + N <= t.cols) {
+        words_t v;
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) v[e] = w[e];
+        *reinterpret_cast<words_t*>(o) = v;
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
@@ -58,7 +62,7 @@ __device__ __forceinline__ void store_words(const F8Out& t, bool vec, int r, int
 template <bool BF>
 __device__ __forceinline__ void store4(const F8Out& t, int r, int c, const f32x4_t& v) {
     const unsigned w[2] = {narrow2<BF>(v[0], v[1]), narrow2<BF>(v[2], v[3])};
-    store_words<4>(t, t.vec, r, c, w);
+    store_words<4>(t, r, c, w);
 }
 // A 32 x 32 accumulator: register 4 g + e of lane (r, h) is column 8 g + 4 h + e of row r.  The lane pairs (r, 0), (r, 1) trade
 // halves, so that lane (r, h) holds the eight columns 8 (g + h).. and a row leaves in pieces of 32 bytes, not 16.
@@ -73,16 +77,21 @@ __device__ __forceinline__ void store32(const F8Out& t, int r, int c, int h, con
             w[e] = (unsigned)x[0];
             w[2 + e] = (unsigned)x[1];
         }
-        store_words<8>(t, t.vec8, r, c + 8 * (g + h), w);
+        store_words<8>(t, r, c + 8 * (g + h), w);
     }
 }
 
+// workgroups go round the eight XCDs: neighbouring tiles, which share rows, to the L2 of one
+__device__ __forceinline__ int logical_tile() {
+    return (gridDim.x & 7) == 0 ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
+}
+
 // b's rows are the matrix instruction's rows: a lane then holds four neighbouring columns of one output row
-template <int MT, int NT, int WM, int WN, bool BF>
+template <int MT, int NT, int WM, int WN, int S, bool BF>
 __global__ void __launch_bounds__(WM * WN * 64) f8_matmul_tile_kernel(F8MatmulArgs p) {
-    using T = F8Tile<MT, NT, WM, WN>;
+    using T = F8Tile<MT, NT, WM, WN, S>;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int tile = blockIdx.x;
+    const int tile = logical_tile();
     const int ti = tile % p.ta, tj = tile / p.ta;
     const long long i0 = (long long)ti * T::QR, j0 = (long long)tj * T::XR;
     F8Src x{p.b.codes + j0 * p.b.stride, p.b.scales + j0 * p.b.sstride, (unsigned)p.b.stride, (unsigned)p.b.sstride, (int)min((long long)T::XR - 1, p.b.n - 1 - j0)};
@@ -92,21 +101,23 @@ __global__ void __launch_bounds__(WM * WN * 64) f8_matmul_tile_kernel(F8MatmulAr
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    T::run(acc, smem, x, q, p.nblk);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave / WN, wn = wave % WN, frow = lane & 15, fq = lane >> 4;
+    T t;
+    t.init(smem, p.nblk);
+    t.aim(x, q);
+    t.run(acc);
+    const int frow = t.lane & 15, fq = t.lane >> 4;
     const F8Out o = out_tile(p, i0, j0);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-            store4<BF>(o, (wn * NT + n) * 16 + frow, (wm * MT + m) * 16 + fq * 4, acc[m][n]);
+            store4<BF>(o, (t.wn * NT + n) * 16 + frow, (t.wm * MT + m) * 16 + fq * 4, acc[m][n]);
 }
 
 // 256 x 256 tiles, a wave per SIMD: workgroups stay, the first slab of the next tile travels under this one's epilogue.
 // Tiles are numbered in bands of eight along a, and consecutive workgroups go round the XCDs: the 32 tiles of an XCD cover 8 x 4,
 // twelve operand panels for its L2.
-// 8192^3: 455 us, 2.42 PFLOP/s; 4096 x 8192 x 8192: 198 us, 2.78; 4096^3: 61 us, 2.24 (tiles of 128 x 128: 585, 292, 71 us).
+// 8192^3: 455 us, 2.42 PFLOP/s; 4096 x 8192 x 8192: 198 us, 2.78; 4096^3: 61 us, 2.24 (8192^3 in tiles of 128 x 128: 585 us).
 // The matrix pipe alone reaches 4.9 PFLOP/s on registers, with the operands' way through LDS the chip's power is the limit.
 template <bool BF>
 __global__ void __launch_bounds__(256, 1) f8_matmul_big_kernel(F8MatmulArgs p) {
@@ -114,7 +125,7 @@ __global__ void __launch_bounds__(256, 1) f8_matmul_big_kernel(F8MatmulArgs p) {
     F8Big t;
     t.init(smem, p.nblk);
     const int tiles = p.ta * p.tb;
-    const int logical = (gridDim.x & 7) == 0 ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
+    const int logical = logical_tile();
     long long i0 = 0, j0 = 0;
     auto aim = [&](int tile) {
         const int band = tile / (8 * p.tb), in = tile - band * 8 * p.tb, rows = min(8, p.ta - band * 8);
@@ -147,59 +158,57 @@ __global__ void __launch_bounds__(256, 1) f8_matmul_big_kernel(F8MatmulArgs p) {
     }
 }
 
-// Few rows of a: 16 rows of b per workgroup, its eight waves take every eighth block of K each and add up through LDS.
-template <int AT, bool BF>
-__global__ void __launch_bounds__(512) f8_matmul_rows_kernel(F8MatmulArgs p) {
-    __shared__ f32x4_t part[8][AT][64];
-    const int lane = threadIdx.x & 63;
+// Few rows of a: (16 NT) rows of a x (16 MT) rows of b per workgroup.  Its W waves share K, each with a ring of its own and no
+// barrier, and add up through LDS.  1 x 4096 x 4096: 5.0 us; 64 x 4096 x 4096: 5.8 us, 2.9 TB/s of b; 128 x 4096 x 4096: 6.8 us.
+template <int MT, int NT, int W, int S, bool BF>
+__global__ void __launch_bounds__(W * 64) f8_matmul_split_kernel(F8MatmulArgs p) {
+    using T = F8Tile<MT, NT, 1, 1, S, true>;
+    extern __shared__ __align__(16) unsigned char smem[];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int frow = lane & 15, fq = lane >> 4;
-    const long long j0 = (long long)blockIdx.x * 16, i0 = (long long)blockIdx.y * (AT * 16);
-    const long long jr = min(j0 + frow, p.b.n - 1);
-    const unsigned char* xp = p.b.codes + jr * p.b.stride + fq * 16;
-    const unsigned char* xs = p.b.scales + jr * p.b.sstride;
-    const unsigned char* ap[AT];
-    const unsigned char* as[AT];
-    f32x4_t acc[AT];
+    const int tile = logical_tile();
+    const long long i0 = (long long)(tile % p.ta) * T::QR, j0 = (long long)(tile / p.ta) * T::XR;
+    const int each = ((p.nblk + W - 1) / W + 3) & ~3;   // whole scale words
+    const int kb = wave * each, nblk = min(each, p.nblk - kb);
+    f32x4_t acc[MT][NT];
 #pragma unroll
-    for (int t = 0; t < AT; ++t) {
-        const long long ir = min(i0 + t * 16 + frow, p.a.n - 1);
-        ap[t] = p.a.codes + ir * p.a.stride + fq * 16;
-        as[t] = p.a.scales + ir * p.a.sstride;
-        acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    T t;
+    t.init(smem + wave * T::LDS, nblk);
+    if (nblk > 0) {
+        t.aim(F8Src{p.b.codes + j0 * p.b.stride + (size_t)kb * 128, p.b.scales + j0 * p.b.sstride + kb, (unsigned)p.b.stride, (unsigned)p.b.sstride, (int)min((long long)T::XR - 1, p.b.n - 1 - j0)},
+              F8Src{p.a.codes + i0 * p.a.stride + (size_t)kb * 128, p.a.scales + i0 * p.a.sstride + kb, (unsigned)p.a.stride, (unsigned)p.a.sstride, (int)min((long long)T::QR - 1, p.a.n - 1 - i0)});
+        t.run(acc);
     }
-    for (int kb = wave; kb < p.nblk; kb += 8) {
-        const size_t o = (size_t)kb * 128;
-        const i32x8_t x = join8(*reinterpret_cast<const i32x4_t*>(xp + o), *reinterpret_cast<const i32x4_t*>(xp + o + 64));
-        const int sx = xs[kb];
+    __syncthreads();   // the rings make room for the sums
+    f32x4_t* part = reinterpret_cast<f32x4_t*>(smem);   // [wave][MT][NT][64]
+    static_assert(W * MT * NT * 1024 <= W * T::LDS, "the sums take the rings' place");
 #pragma unroll
-        for (int t = 0; t < AT; ++t) {
-            const i32x8_t a = join8(*reinterpret_cast<const i32x4_t*>(ap[t] + o), *reinterpret_cast<const i32x4_t*>(ap[t] + o + 64));
-            acc[t] = mfma_f8<0>(x, a, acc[t], sx, (int)as[t][kb]);
-        }
-    }
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int t = 0; t < AT; ++t) part[wave][t][lane] = acc[t];
+        for (int n = 0; n < NT; ++n) part[((wave * MT + m) * NT + n) * 64 + t.lane] = acc[m][n];
     __syncthreads();
     const F8Out o = out_tile(p, i0, j0);
-    for (int t = wave; t < AT; t += 8) {
-        f32x4_t v = part[0][t][lane];
+    const int frow = t.lane & 15, fq = t.lane >> 4;
+    for (int f = wave; f < MT * NT; f += W) {
+        f32x4_t v = part[f * 64 + t.lane];
 #pragma unroll
-        for (int w = 1; w < 8; ++w) v += part[w][t][lane];
-        store4<BF>(o, t * 16 + frow, fq * 4, v);
+        for (int w = 1; w < W; ++w) v += part[(w * MT * NT + f) * 64 + t.lane];
+        store4<BF>(o, (f % NT) * 16 + frow, (f / NT) * 16 + fq * 4, v);
     }
 }
 
-template <int MT, int NT, int WM, int WN, bool BF>
+template <int MT, int NT, int WM, int WN, int S, bool BF>
 static hipError_t launch_tile(F8MatmulArgs& p, hipStream_t s) {
-    using T = F8Tile<MT, NT, WM, WN>;
+    using T = F8Tile<MT, NT, WM, WN, S>;
     p.ta = (int)((p.a.n + T::QR - 1) / T::QR);
     p.tb = (int)((p.b.n + T::XR - 1) / T::XR);
     if (T::LDS > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_matmul_tile_kernel<MT, NT, WM, WN, BF>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_matmul_tile_kernel<MT, NT, WM, WN, S, BF>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((f8_matmul_tile_kernel<MT, NT, WM, WN, BF>), dim3((unsigned)((long long)p.ta * p.tb)), dim3(T::THREADS), T::LDS, s, p);
+    hipLaunchKernelGGL((f8_matmul_tile_kernel<MT, NT, WM, WN, S, BF>), dim3((unsigned)((long long)p.ta * p.tb)), dim3(T::THREADS), T::LDS, s, p);
     return hipGetLastError();
 }
 template <bool BF>
@@ -212,19 +221,47 @@ static hipError_t launch_big(F8MatmulArgs& p, int num_cu, hipStream_t s) {
     hipLaunchKernelGGL(f8_matmul_big_kernel<BF>, dim3((unsigned)(tiles < num_cu ? tiles : num_cu)), dim3(256), F8Big::LDS, s, p);
     return hipGetLastError();
 }
+template <int MT, int NT, int W, int S, bool BF>
+static hipError_t launch_split(F8MatmulArgs& p, hipStream_t s) {
+    using T = F8Tile<MT, NT, 1, 1, S, true>;
+    p.ta = (int)((p.a.n + T::QR - 1) / T::QR);
+    p.tb = (int)((p.b.n + T::XR - 1) / T::XR);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_matmul_split_kernel<MT, NT, W, S, BF>), hipFuncAttributeMaxDynamicSharedMemorySize, W * T::LDS);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((f8_matmul_split_kernel<MT, NT, W, S, BF>), dim3((unsigned)((long long)p.ta * p.tb)), dim3(W * 64), W * T::LDS, s, p);
+    return hipGetLastError();
+}
 template <bool BF>
 static hipError_t launch_t(F8MatmulArgs& p, int num_cu, hipStream_t s) {
     const long long m = p.a.n, n = p.b.n;
-    if (m <= 64) {
-        const int at = m <= 16 ? 1 : m <= 32 ? 2 : 4;
-        const dim3 grid((unsigned)((n + 15) / 16), 1);
-        if (at == 1) hipLaunchKernelGGL((f8_matmul_rows_kernel<1, BF>), grid, dim3(512), 0, s, p);
-        else if (at == 2) hipLaunchKernelGGL((f8_matmul_rows_kernel<2, BF>), grid, dim3(512), 0, s, p);
-        else hipLaunchKernelGGL((f8_matmul_rows_kernel<4, BF>), grid, dim3(512), 0, s, p);
-        return hipGetLastError();
+    const long long nb = p.nblk, t64 = ((m + 63) / 64) * ((n + 63) / 64);
+    // One launch of T tiles takes as many rounds as it has times the chip's places for their workgroups.  A round's time was
+    // measured as (fixed part) + (part per block of K), in units of 10 ns, e.g. 33.8 us for 2048 x 4096 x 4096 in tiles of 128 x 128.
+    const auto cost = [&](int tm, int tn, int places, long long fixed, long long block) {
+        const long long tiles = ((m + tm - 1) / tm) * ((n + tn - 1) / tn), at_once = (long long)places * num_cu;
+        return (tiles + at_once - 1) / at_once * (fixed + block * nb);
+    };
+    const auto least = [](std::initializer_list<long long> c) { return std::min_element(c.begin(), c.end()) - c.begin(); };
+    // A workgroup gets 57 B/ns from the caches at best, so where tiles are few the waves share K and the tiles are small (us in tiles
+    // of 32 x 32, 64 x 32 and 64 x 64, and of 64 x 64 whose waves share slabs: 64 x 4096 x 4096 5.8, 6.5, 8.0, 9.7; 128 x 4096 x 4096 8.7, 6.8, 7.9,
+    // 10.2; 1 x 4096 x 4096 in 16 x 16 5.0, else 6.0).  With more tiles than CUs slabs that are shared win (512 x 4096 x 4096 23.2 in 64 x 32, 15.7), and
+    // for few rows of a already where the tiles fill most of the chip: b then streams from memory (16 x 12288 x 4096 12.1, 10.0)
+    if (t64 <= num_cu && (m > 64 || 4 * t64 < 3 * num_cu)) {
+        switch (least({cost(16, 16, 1, 80, 7), cost(32, 32, 1, 70, 12), cost(64, 32, 1, 190, 14), cost(64, 64, 1, 250, 19)})) {
+            case 0: return launch_split<1, 1, 8, 3, BF>(p, s);
+            case 1: return launch_split<2, 2, 8, 2, BF>(p, s);
+            case 2: return launch_split<2, 4, 4, 3, BF>(p, s);
+            default: return launch_split<4, 4, 4, 2, BF>(p, s);
+        }
     }
-    if (((m + 255) / 256) * ((n + 255) / 256) >= num_cu) return launch_big<BF>(p, num_cu, s);
-    return launch_tile<4, 4, 2, 2, BF>(p, s);
+    // (tiles of 64 x 64, 128 x 128 of one workgroup per CU and of two, 256 x 256: 512 x 4096 x 4096 15.7, 19.9, 25.5, 40.0;
+    // 1024 x 4096 x 4096 30.6, 22.4, 28.4, 41.4; 2048 x 4096 x 4096 72.6, 43.3, 35.5, 43.3; 4096^3 149, 94, 72, 56)
+    switch (least({t64 <= num_cu ? 200 + 25 * nb : cost(64, 64, 2, 200, 36), cost(128, 128, 1, 330, 55), cost(128, 128, 2, 500, 90), cost(256, 256, 1, 650, 166)})) {
+        case 0: return launch_tile<2, 2, 2, 2, 4, BF>(p, s);
+        case 1: return launch_tile<4, 2, 2, 4, 4, BF>(p, s);
+        case 2: return launch_tile<4, 4, 2, 2, 2, BF>(p, s);
+        default: return launch_big<BF>(p, num_cu, s);
+    }
 }
 
 hipError_t launch_f8_matmul(const F8Mat& a, const F8Mat& b, int k, void* out, int out_dtype, long long out_stride, int num_cu, hipStream_t s) {
@@ -235,8 +272,6 @@ hipError_t launch_f8_matmul(const F8Mat& a, const F8Mat& b, int k, void* out, in
     p.nblk = f8_blocks(k);
     p.out = static_cast<unsigned short*>(out);
     p.ostride = out_stride;
-    p.vec = ((uintptr_t)out & 7) == 0 && (out_stride & 3) == 0;
-    p.vec8 = ((uintptr_t)out & 15) == 0 && (out_stride & 7) == 0;
     return out_dtype == 2 ? launch_t<true>(p, num_cu, s) : launch_t<false>(p, num_cu, s);
 }
 

@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(512) f8_scan_kernel(F8ScanArgs A) {
 // ---- tile kernel: 256 rows x TQ queries per workgroup, a slice of the rows each ----
 template <int MT, int NT, int WM, int WN, int R>
 __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, MfmaParams P) {
-    using T = F8Tile<MT, NT, WM, WN>;
+    using T = F8Tile<MT, NT, WM, WN, 3>;
     static_assert(T::XR == 256 && T::WAVES == 8, "row tile and folds of the 16-bit kernels");
     extern __shared__ __align__(16) unsigned char smem[];
     float* thr_l = reinterpret_cast<float*>(smem + T::LDS);
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, 
     unsigned* flag_l = kept_l + 256;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave / WN, wn = wave % WN, frow = lane & 15, fq = lane >> 4;
+    const int frow = lane & 15, fq = lane >> 4;
     int logical = blockIdx.x;
     if ((gridDim.x & 7) == 0) logical = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     const int slice = logical / P.nqt, qt = logical % P.nqt;
@@ -521,20 +521,26 @@ __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, 
     __syncthreads();
     const long long seg_mask = (1ll << V.X.seg_shift) - 1;
     const F8Src qsrc{q.codes + (size_t)q0 * q.stride, q.scales + (size_t)q0 * q.sstride, (unsigned)q.stride, (unsigned)q.sstride, (int)min((long long)T::QR - 1, q.n - 1 - q0)};
-    unsigned tiles_done = 0;
-    for (long long row0 = r_begin; row0 < r_end; row0 += 256) {
+    T t;
+    t.init(smem, V.X.ld / kF8Block);
+    auto aim = [&](long long row0) __attribute__((always_inline)) {
         const long long seg = row0 >> V.X.seg_shift, off = row0 & seg_mask;
+        t.aim(F8Src{static_cast<const unsigned char*>(V.X.segs[seg]) + off * V.X.ld, static_cast<const unsigned char*>(V.ssegs[seg]) + off * V.sld,
+                    (unsigned)V.X.ld, (unsigned)V.sld, (int)min(255ll, r_end - 1 - row0)}, qsrc);
+    };
+    unsigned tiles_done = 0;
+    if (r_begin < r_end) aim(r_begin);
+    for (long long row0 = r_begin; row0 < r_end; row0 += 256) {
         const long long left = r_end - row0;
-        const F8Src xsrc{static_cast<const unsigned char*>(V.X.segs[seg]) + off * V.X.ld, static_cast<const unsigned char*>(V.ssegs[seg]) + off * V.sld,
-                         (unsigned)V.X.ld, (unsigned)V.sld, (int)min(255ll, left - 1)};
         f32x4_t acc[MT][NT];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        T::run(acc, smem, xsrc, qsrc, V.X.ld / kF8Block);
-        if (left >= 256) filter_tile<MT, NT, true>(acc, wm * MT * 16, wn * NT * 16, frow, fq, row0, 256, cand, thr_l, cnt_l, flag_l);
-        else filter_tile<MT, NT, false>(acc, wm * MT * 16, wn * NT * 16, frow, fq, row0, (int)left, cand, thr_l, cnt_l, flag_l);
+        t.run(acc);
+        if (row0 + 256 < r_end) aim(row0 + 256);   // its first slabs travel under the filter
+        if (left >= 256) filter_tile<MT, NT, true>(acc, t.wm * MT * 16, t.wn * NT * 16, frow, fq, row0, 256, cand, thr_l, cnt_l, flag_l);
+        else filter_tile<MT, NT, false>(acc, t.wm * MT * 16, t.wn * NT * 16, frow, fq, row0, (int)left, cand, thr_l, cnt_l, flag_l);
         __syncthreads();
         ++tiles_done;
         // fold after row tiles 1, 4, 16, ... of the slice and whenever a candidate buffer is half full
@@ -767,7 +773,7 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
         p->parts = p->nslices;
         p->grid_x = p->nqt * p->nslices;
         p->threads = 512;
-        p->lds = (p->tq == 256 ? (size_t)F8Pp::LDS : (size_t)2 * (256 + p->tq) * 128) + EPI_LDS_BYTES;
+        p->lds = (size_t)(p->tq == 256 ? F8Pp::LDS : p->tq == 128 ? F8Tile<4, 4, 4, 2, 3>::LDS : F8Tile<2, 4, 8, 1, 3>::LDS) + EPI_LDS_BYTES;
         p->cand_bytes = (size_t)p->grid_x * 256 * CAND_CAP * sizeof(skey_t);
         // scores every slice publishes per query: enough that the kp-th largest of all of them exists and is tight (mfma.hip)
         int m = (int)((std::max<long long>(64, (long long)p->kp * 5 / 4) + p->nslices - 1) / p->nslices);
