@@ -13,7 +13,9 @@ CSRC = Path(__file__).resolve().parent / "csrc"
 LIB = CSRC / "libssmi.so"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
-         "-fno-gpu-rdc", "-DNDEBUG"]
+         "-fno-gpu-rdc", "-DNDEBUG",
+         # no packed fp32 arithmetic: some forms of it have given wrong results (the host pass warns of an unknown feature)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale(target: Path, deps) -> bool:
