@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, 
         __syncthreads();
         ++tiles_done;
         // fold after row tiles 1, 4, 16, ... of the slice and whenever a candidate buffer is half full
-        if (((tiles_done & (tiles_done - 1)) == 0 && (tiles_done & P.fold_mask)) || *flag_l) {
+        if (row0 + 256 < r_end && (((tiles_done & (tiles_done - 1)) == 0 && (tiles_done & P.fold_mask)) || *flag_l)) {   // (the end folds anyway)
             fold_queries<R>(wave, q0, P, slice, cand, thr_l, cnt_l, kept_l);
             if (lane < 32) {   // the k-th score of any slice bounds the final one: the slices share the highest (mfma.hip)
                 const int ql = wave + 8 * lane;
@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(512, 2) f8_search_big_kernel(F8View V, F8Mat q
         else filter_big<false>(acc, t.wm * 128, t.wn * 64, lane, row0, (int)left, cand, thr_l, cnt_l, flag_l, 0);
         __syncthreads();
         ++tiles_done;
-        const bool fold_due = ((tiles_done & (tiles_done - 1)) == 0 && (tiles_done & P.fold_mask)) || *flag_l;
+        const bool fold_due = row0 + 256 < r_end && (((tiles_done & (tiles_done - 1)) == 0 && (tiles_done & P.fold_mask)) || *flag_l);   // (the end folds anyway)
         if (xstate && !fold_due) {
             if (xstate == 1) push_bounds(lane); else pull_thr(lane);
             xstate = xstate == 1 ? 2 : 0;
