@@ -54,6 +54,8 @@ def search(X, Q, k):
     I = np.full((len(Q), k), -1, dtype=np.int64)
     for i, s in enumerate(S):
         ids = np.flatnonzero(~np.isnan(s))
+        if len(ids) > k:
+            ids = ids[s[ids] >= np.partition(s[ids], len(ids) - k)[len(ids) - k]]   # (only what can be among them is sorted)
         order = ids[np.lexsort((ids, -s[ids]))][:k]
         D[i, :len(order)] = s[order].astype(np.float32)
         I[i, :len(order)] = order

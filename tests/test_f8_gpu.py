@@ -435,3 +435,58 @@ def test_refusals_of_a_live_index(ssa):
         index.add(ssa.quantize_f8(q[:, :100]))
     with pytest.raises(RuntimeError, match="Flat"):
         ssa.IndexIVFFlat(None, 128, 4, storage="f8")
+
+
+# one size at least for every tile (16 x 16 to 256 x 256), whole and ragged, and every length of their rings
+@pytest.mark.parametrize("m,n", [(1, 4096), (16, 200), (97, 1000), (64, 4090), (128, 4096), (250, 4090), (512, 4096), (1000, 4090), (2040, 4096), (4090, 4096), (4100, 8200)])
+@pytest.mark.parametrize("k", [100, 256, 300, 512, 513, 700, 1100])
+def test_product_in_every_tile(ssa, m, n, k):
+    torch.manual_seed(SALT + m + n + k)
+    # -1, 0 and 1 times a power of two a row: every product and sum is exact, in whatever order
+    xa, xb = (torch.randint(-1, 2, (c, k), device="cuda").float() for c in (m, n))
+    xa[:, 0] = xb[:, 0] = 1
+    sa, sb = (torch.exp2(torch.randint(-3, 4, (c, 1), device="cuda").float()) for c in (m, n))
+    a, b = ssa.quantize_f8(xa * sa), ssa.quantize_f8(xb * sb)
+    want = ((xa.double() @ xb.double().T) * sa.double() * sb.double().T).bfloat16()
+    assert torch.equal(ssa.matmul_f8(a, b), want)
+
+
+@pytest.mark.parametrize("n,d,nq,k", [(70000, 130, 129, 10), (140000, 64, 300, 49), (66000, 200, 700, 100), (40000, 128, 1025, 1), (513, 400, 200, 48), (20000, 1100, 150, 300),
+                                      (70000, 64, 100, 10), (70000, 520, 20, 30)])
+def test_search_of_large_batches_over_many_row_tiles(ssa, n, d, nq, k):
+    X, Q = unit_rows(n, d, SALT + n + d), unit_rows(nq, d, SALT + nq)
+    index = filled(ssa, cuda(X))
+    check_search(*index.search(Q, k), plain.round_rows(X), plain.round_rows(Q), k)
+
+
+@pytest.mark.parametrize("nq", [20, 100, 300])
+@pytest.mark.parametrize("k", [10, 60])
+def test_search_of_rows_that_get_better_and_better(ssa, nq, k):
+    """Every row tile beats all before it: each threshold is late.  The values are exact, with many equal ones."""
+    n, d = 80000, 256
+    X = np.zeros((n, d), np.float32)
+    X[:, :5] = (np.arange(n)[:, None] // 160 >> np.arange(8, -1, -2) & 3) * 4.0 ** np.arange(4, -1, -1)   # digits of base 4 that add up to i // 160
+    X[:, 128:133] = X[:, :5]
+    Q = np.zeros((nq, d), np.float32)
+    Q[np.arange(nq) % 3 != 1, :5] = 1
+    Q[np.arange(nq) % 3 != 0, 128:133] = 1
+    Q[:, 200] = np.arange(nq)   # (no row answers to it)
+    check_search(*filled(ssa, X).search(Q, k), plain.round_rows(X), plain.round_rows(Q), k)
+
+
+def test_large_batches_over_many_segments(ssa, monkeypatch):
+    monkeypatch.setenv("SSMI_SEG_SHIFT", "8")
+    X, Q = unit_rows(20000, 300, SALT + 20), unit_rows(310, 300, SALT + 21)
+    index = filled(ssa, X)
+    for nq in (16, 128, 310):
+        check_search(*index.search(Q[:nq], 12), plain.round_rows(X), plain.round_rows(Q[:nq]), 12)
+
+
+@pytest.mark.parametrize("nq", [12, 100, 300])
+def test_large_batches_of_rows_and_queries_that_are_not_finite(ssa, nq):
+    X, Q = unit_rows(3000, 256, SALT + 22), unit_rows(nq, 256, SALT + 23)
+    X[::2, 7] = np.nan    # half the rows of every tile
+    X[1:600:2, 200] = np.inf
+    Q[3, 0] = np.nan
+    with np.errstate(invalid="ignore"):
+        check_search(*filled(ssa, X).search(Q, 10), plain.round_rows(X), plain.round_rows(Q), 10)
