@@ -491,6 +491,36 @@ __global__ void __launch_bounds__(512) f8_scan_kernel(F8ScanArgs A) {
     finish_query(V, qs, qsc, ids, kp, A.k, A.D, A.I, A.id_offset, A.min_ord, score, cid);
 }
 
+// the k-th score of any slice bounds the final one: the slices share the highest (mfma.hip).  A wave's own queries, as in the folds
+__device__ __forceinline__ void share_thresholds(int wave, int lane, int q0, const MfmaParams& P, float* thr_l) {
+    const int ql = wave + 8 * lane;
+    if (lane < 32 && q0 + ql < P.nq) {
+        const float t = thr_l[ql];
+        const unsigned mine = t > SSMI_NEG_MAX ? f32_to_ord(t) : 0u;
+        const unsigned seen = atomicMax(&P.gthr[q0 + ql], mine);
+        if (seen > mine) thr_l[ql] = ord_to_f32(seen);
+    }
+}
+
+// ---- first thresholds of a slice ----
+// No list exists yet and every row of its first tile would pass the filter, go to memory and be sorted.  The tile's rows are taken in 64
+// groups of four; a group's largest score is a row, so the kp-th largest of a query's 64 group maxima (kp <= 64) has kp rows at or above
+// it and bounds the kp-th score from below.  About 30 rows of 256 pass it at kp = 26.  The slices share the highest, as behind a fold.
+static constexpr int kSeedPitch = 65;   // words of a query's maxima: lanes that hold neighbouring queries write to banks of their own
+template <int TQ>
+__device__ __forceinline__ void seed_thresholds(const float* maxima, int wave, int lane, int q0, const MfmaParams& P, float* thr_l) {
+#pragma unroll 1
+    for (int ql = wave; ql < TQ; ql += 8) {
+        if (q0 + ql >= P.nq) break;
+        WaveSort32<1> t;
+        t.v[0] = f32_to_ord(maxima[ql * kSeedPitch + lane]);
+        t.sort_desc();
+        const float kth = ord_to_f32(t.kth(P.k));
+        if (lane == 0) lds_store(reinterpret_cast<unsigned*>(&thr_l[ql]), __float_as_uint(fmaxf(kth, P.thr_floor)));
+    }
+    share_thresholds(wave, lane, q0, P, thr_l);
+}
+
 // ---- tile kernel: 256 rows x TQ queries per workgroup, a slice of the rows each ----
 template <int MT, int NT, int WM, int WN, int R>
 __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, MfmaParams P) {
@@ -538,6 +568,23 @@ __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, 
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         t.run(acc);
+        if (tiles_done == 0 && P.k <= 64) {
+            float* maxima = reinterpret_cast<float*>(smem);   // (the ring is free)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    // (no NaN may enter the sort, and no row behind the last)
+                    float v = SSMI_NEG_MAX;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if ((t.wm * MT + m) * 16 + fq * 4 + i < left) v = vmax2(v, acc[m][n][i]);
+                    maxima[((t.wn * NT + n) * 16 + frow) * kSeedPitch + (t.wm * MT + m) * 4 + fq] = v;
+                }
+            __syncthreads();
+            seed_thresholds<T::QR>(maxima, wave, lane, q0, P, thr_l);
+            __syncthreads();
+        }
         if (row0 + 256 < r_end) aim(row0 + 256);   // its first slabs travel under the filter
         if (left >= 256) filter_tile<MT, NT, true>(acc, t.wm * MT * 16, t.wn * NT * 16, frow, fq, row0, 256, cand, thr_l, cnt_l, flag_l);
         else filter_tile<MT, NT, false>(acc, t.wm * MT * 16, t.wn * NT * 16, frow, fq, row0, (int)left, cand, thr_l, cnt_l, flag_l);
@@ -546,15 +593,7 @@ __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, 
         // fold after row tiles 1, 4, 16, ... of the slice and whenever a candidate buffer is half full
         if (row0 + 256 < r_end && (((tiles_done & (tiles_done - 1)) == 0 && (tiles_done & P.fold_mask)) || *flag_l)) {   // (the end folds anyway)
             fold_queries<R>(wave, q0, P, slice, cand, thr_l, cnt_l, kept_l);
-            if (lane < 32) {   // the k-th score of any slice bounds the final one: the slices share the highest (mfma.hip)
-                const int ql = wave + 8 * lane;
-                if (q0 + ql < P.nq) {
-                    const float t = thr_l[ql];
-                    const unsigned mine = t > SSMI_NEG_MAX ? f32_to_ord(t) : 0u;
-                    const unsigned seen = atomicMax(&P.gthr[q0 + ql], mine);
-                    if (seen > mine) thr_l[ql] = ord_to_f32(seen);
-                }
-            }
+            share_thresholds(wave, lane, q0, P, thr_l);
             __syncthreads();
             if (tid == 0) *flag_l = 0;
         }
@@ -566,42 +605,14 @@ __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, 
 // ---- large batches: 256 rows x 256 queries on the contraction of f8_pp.h ----
 // Threshold filter over a wave's 128 x 64 accumulators (acc[m][n][4 g + e]: row row_base + 32 m + 8 g + 4 h + e, query q_base + 32 n + r
 // of lane (r, h)): as filter_tile of the 16-bit kernels, one column maximum first, survivors one by one.
-// seed: first row tile of a slice, whole, and kp <= 64: no list exists yet and every row would pass.  The lane's 64 rows
-// of a query are taken in pairs and the 32 maxima sorted; at least c = ceil(kp / 2) rows of each of the two lanes of a column reach the
-// lane's c-th, so the smaller of the two has kp of this wave's rows at or above it and may serve as threshold for this tile.
 template <bool FULL>
 __device__ __forceinline__ void filter_big(const F8Pp::Acc& acc, int row_base, int q_base, int lane, long long row0, int rows_valid, skey_t* cand,
-                                           const float* thr_l, unsigned* cnt_l, unsigned* flag_l, int seed) {
+                                           const float* thr_l, unsigned* cnt_l, unsigned* flag_l) {
     const int r = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
         const int ql = q_base + 32 * n + r;
-        float thr = thr_l[ql];
-        if (FULL && seed) {
-            float v[32];
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const f32x16_t a = acc[m][n];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[m * 8 + i] = vmax3(a[2 * i], a[2 * i + 1], SSMI_NEG_MAX);   // (no NaN may enter the sort: it would double its partner)
-            }
-#pragma unroll
-            for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-                for (int st = size >> 1; st >= 1; st >>= 1)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if ((i & st) == 0) {
-                            const float a = v[i], b = v[i + st];
-                            const bool desc = (i & size) == 0 || size == 32;
-                            v[i] = desc ? fmaxf(a, b) : fminf(a, b);
-                            v[i + st] = desc ? fminf(a, b) : fmaxf(a, b);
-                        }
-            float t = v[0];
-#pragma unroll
-            for (int i = 1; i < 32; ++i) t = i < seed ? v[i] : t;
-            thr = fmaxf(thr, fminf(t, __int_as_float(xor_lane<32>(__float_as_int(t)))));
-        }
+        const float thr = thr_l[ql];
         float mm[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
@@ -680,7 +691,6 @@ __global__ void __launch_bounds__(512, 2) f8_search_big_kernel(F8View V, F8Mat q
             if (seen && ord_to_f32(seen) > thr_l[ql]) lds_store(reinterpret_cast<unsigned*>(&thr_l[ql]), __float_as_uint(ord_to_f32(seen)));
         }
     };
-    const int seed_c = P.k <= 64 ? (P.k + 1) / 2 : 0;
     unsigned tiles_done = 0;
     int xstate = 0;
     if (r_begin < r_end) aim(r_begin);
@@ -695,10 +705,24 @@ __global__ void __launch_bounds__(512, 2) f8_search_big_kernel(F8View V, F8Mat q
                 for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
         t.run(acc);
         const long long left = r_end - row0;
+        int lane = t.lane;
+        asm volatile("" : "+v"(lane));   // (addresses are made here and not ahead of the loop, whose registers are all taken)
+        if (tiles_done == 0 && P.k <= 64 && left >= 256) {
+            float* maxima = reinterpret_cast<float*>(smem) + (t.wn * 64 + (lane & 31)) * kSeedPitch + t.wm * 32 + (lane >> 5);   // (the ring is free)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)   // (no NaN may enter the sort)
+                        maxima[n * 32 * kSeedPitch + (m * 4 + g) * 2] = vmax3(vmax3(acc[m][n][g * 4], acc[m][n][g * 4 + 1], SSMI_NEG_MAX), acc[m][n][g * 4 + 2], acc[m][n][g * 4 + 3]);
+            __syncthreads();
+            seed_thresholds<256>(reinterpret_cast<const float*>(smem), t.wave, lane, q0, P, thr_l);
+            __syncthreads();
+        }
         if (row0 + 256 < r_end) aim(row0 + 256);
-        const int lane = t.lane;
-        if (left >= 256) filter_big<true>(acc, t.wm * 128, t.wn * 64, lane, row0, 256, cand, thr_l, cnt_l, flag_l, tiles_done == 0 ? seed_c : 0);
-        else filter_big<false>(acc, t.wm * 128, t.wn * 64, lane, row0, (int)left, cand, thr_l, cnt_l, flag_l, 0);
+        if (left >= 256) filter_big<true>(acc, t.wm * 128, t.wn * 64, lane, row0, 256, cand, thr_l, cnt_l, flag_l);
+        else filter_big<false>(acc, t.wm * 128, t.wn * 64, lane, row0, (int)left, cand, thr_l, cnt_l, flag_l);
         __syncthreads();
         ++tiles_done;
         const bool fold_due = row0 + 256 < r_end && (((tiles_done & (tiles_done - 1)) == 0 && (tiles_done & P.fold_mask)) || *flag_l);   // (the end folds anyway)
@@ -710,13 +734,7 @@ __global__ void __launch_bounds__(512, 2) f8_search_big_kernel(F8View V, F8Mat q
             fold_queries<R>(t.wave, q0, P, slice, cand, thr_l, cnt_l, kept_l);
             xstate = P.gtop ? 1 : 0;
             __syncthreads();
-            const int ql = t.wave + 8 * lane;
-            if (lane < 32 && q0 + ql < P.nq) {
-                const float th = thr_l[ql];
-                const unsigned mine = th > SSMI_NEG_MAX ? f32_to_ord(th) : 0u;
-                const unsigned seen = atomicMax(&P.gthr[q0 + ql], mine);
-                if (seen > mine) thr_l[ql] = ord_to_f32(seen);
-            }
+            share_thresholds(t.wave, lane, q0, P, thr_l);
             __syncthreads();
             if (threadIdx.x == 0) *flag_l = 0;
         }

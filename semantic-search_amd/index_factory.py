@@ -47,7 +47,7 @@ class IndexConfig:
     pq_bits: int = 8
     is_trained: bool = False
     training_size: int = 0
-    # additive, not serialised: engine options {"storage": "f32"|"f16"|"bf16", "device": int, "devices": [int, ...]}
+    # additive, not serialised: engine options {"storage": "f32"|"f16"|"bf16"|"f8" (Flat), "device": int, "devices": [int, ...]}
     extra: Dict[str, Any] = field(default_factory=dict, repr=False, compare=False)
 
     _KEYS = ("nlist", "nprobe", "hnsw_m", "hnsw_ef_construction", "hnsw_ef_search", "pq_m", "pq_bits",
