@@ -6,7 +6,7 @@ or take an `F8Rows` as it is - for instance what `rms_norm_f8(..., unit=True)` m
 what the reference's embedder does in fp32 before it hands rows to FAISS (core/qwen3_vl_embedding.py:447-448).
 
 All calls work on tensors of a ROCm device, enqueue on its current torch stream, wait for nothing and may be captured into a
-graph.  Argument errors raise ValueError or TypeError, errors of the engine RuntimeError.
+graph; none of them records a gradient.  Argument errors raise ValueError or TypeError, errors of the engine RuntimeError.
 """
 from typing import Optional
 
@@ -196,6 +196,8 @@ def matmul_f8(a: F8Rows, b: F8Rows, out_dtype: torch.dtype = torch.bfloat16, out
     if i != b.device_index:
         raise ValueError(f"matmul_f8: operands on {a.device} and {b.device}")
     if out is not None:
+        if not isinstance(out, torch.Tensor):
+            raise TypeError(f"matmul_f8: out must be a tensor, got {type(out).__name__}")
         out_dtype = out.dtype
     if out_dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"matmul_f8: the output is float16 or bfloat16, not {out_dtype}")

@@ -38,6 +38,8 @@ _HEADER = struct.Struct("<iqqqBi")
 
 def _as_rows(x, d: int, what: str):
     """numpy (n,d) float32, or a torch tensor left where it is."""
+    if isinstance(x, fc.F8Rows):
+        raise RuntimeError(f"{what}: an index over several devices takes plain rows and quantises them itself")
     if isinstance(x, torch.Tensor):
         if x.dim() == 1:
             x = x.reshape(1, -1)

@@ -490,3 +490,87 @@ def test_large_batches_of_rows_and_queries_that_are_not_finite(ssa, nq):
     Q[3, 0] = np.nan
     with np.errstate(invalid="ignore"):
         check_search(*filled(ssa, X).search(Q, 10), plain.round_rows(X), plain.round_rows(Q), 10)
+
+
+def test_an_index_over_several_devices_refuses_rows_that_are_8_bit_already(ssa):
+    rows = ssa.quantize_f8(cuda(unit_rows(5, 128, 3)))
+    index = ssa.IndexFlatIP(128, storage="f8", devices=[0, 0])
+    for call in (lambda: index.add(rows), lambda: index.search(rows, 2)):
+        with pytest.raises(RuntimeError, match="plain rows"):
+            call()
+
+
+def test_the_manager_keeps_8_bit_rows(ssa, tmp_path):
+    """add / search / save / reload / compact of the manager over 8-bit rows: what an index of the rounded rows gives."""
+    from semantic_search_amd.index_manager import SemanticIndex
+    d, n = 96, 600
+    X, q = unit_rows(n, d, SALT + 30), unit_rows(1, d, SALT + 31)[0]
+    make = lambda: SemanticIndex("eight", d, "flat", base_path=tmp_path, check_files_exist=False, storage="f8")  # noqa: E731
+    ix = make()
+    for s in range(0, n, 50):
+        ix.add_vectors(X[s:s + 50], [f"/img/{i}.jpg" for i in range(s, s + 50)], [""] * 50, [(0.0, 0)] * 50)
+    ids = lambda r: [(x.vector_id, x.file_path) for x in r.results]  # noqa: E731
+    _, want = plain.search(plain.round_rows(X), plain.round_rows(q[None]), 20)
+    assert [i for i, _ in ids(ix.search(q, 20))] == want[0].tolist()
+    first = ids(ix.search(q, 20))
+    ix.save()
+    ix.close()
+    ix = make()
+    assert ix._faiss_index.storage == "f8" and ids(ix.search(q, 20)) == first
+    for i in range(0, n, 3):
+        assert ix.db.remove_image(f"/img/{i}.jpg")
+    assert ix.compact()["success"]
+    left = np.array([i for i in range(n) if i % 3])
+    assert ix._faiss_index.storage == "f8" and ix._faiss_index.ntotal == len(left)
+    _, want = plain.search(plain.round_rows(X[left]), plain.round_rows(q[None]), 20)
+    assert [p for _, p in ids(ix.search(q, 20))] == [f"/img/{left[i]}.jpg" for i in want[0]]
+    ix.close()
+
+
+def test_two_graphs_and_eager_products_at_once(ssa):
+    """Products and norms keep nothing between calls: two captured graphs and eager work on three streams do not meet."""
+    torch.manual_seed(SALT + 32)
+    b = ssa.quantize_f8(torch.randn(4096, 1024, device="cuda"))
+    sets = []
+    for m in (1, 40, 700):
+        x = torch.randn(m, 1024, device="cuda").bfloat16()
+        rows, out = ssa.F8Rows.empty(m, 1024, "cuda"), torch.empty(m, 4096, dtype=torch.bfloat16, device="cuda")
+        sets.append((x, rows, out, ssa.matmul_f8(ssa.rms_norm_f8(x), b)))
+
+    def step(s):
+        ssa.rms_norm_f8(s[0], out=s[1])
+        ssa.matmul_f8(s[1], b, out=s[2])
+    torch.cuda.synchronize()
+    graphs = []
+    for s in sets[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step(s)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        for s in sets:
+            s[2].zero_()
+        torch.cuda.synchronize()
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i].replay() if i < 2 else step(sets[2])
+        torch.cuda.synchronize()
+        for s in sets:
+            assert torch.equal(s[2], s[3])
+
+
+def test_one_operand_twice_and_wide_strides(ssa):
+    x = torch.randn(300, 500, device="cuda")
+    a = ssa.quantize_f8(x)
+    s = ssa.matmul_f8(a, a)
+    assert torch.equal(s, s.T.contiguous())
+    # rows far apart in one allocation: every 7th row of a table, by its strides
+    wide = torch.zeros(300 * 7, 512, dtype=torch.uint8, device="cuda")
+    wide_s = torch.zeros(300 * 7, 4, dtype=torch.uint8, device="cuda")
+    wide[::7], wide_s[::7] = a.codes.view(torch.uint8), a.scales
+    far = ssa.F8Rows.from_parts(wide[::7], wide_s[::7], 500)
+    assert far.codes.stride(0) == 7 * 512
+    assert torch.equal(ssa.matmul_f8(far, a), s) and torch.equal(far.dequantize(), a.dequantize())
+    with pytest.raises(TypeError, match="tensor"):
+        ssa.matmul_f8(a, a, out=[1])
