@@ -782,9 +782,13 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
         p->parts = p->grid_x;
         p->kernel = "f8_scan_kernel";
     } else {
-        p->tq = nq <= 64 ? 64 : nq <= 128 ? 128 : 256;
-        p->nqt = (nq + p->tq - 1) / p->tq;
+        // Over few rows narrow tiles of queries win: more workgroups, fewer lists each.  Up to seven rounds of the chip (us in tiles of 64, 128 and
+        // 256 queries: 10000 x 4096, 256 queries 74, 102, 169; 20000 x 4096, 512 queries 147, 175, 180; 100000 x 4096, 256 queries 299, 312, 371, 512
+        // queries 471, 422, 472, 1024 queries 797, 678, 630; 1M x 4096, 256 queries 1809, 1540, 1349)
         const long long tiles = (nrows + 255) / 256;
+        const auto few = [&](int tq) { return tiles * ((nq + tq - 1) / tq) <= 7ll * num_cu; };
+        p->tq = nq <= 64 || few(64) ? 64 : nq <= 128 || few(128) ? 128 : 256;
+        p->nqt = (nq + p->tq - 1) / p->tq;
         const long long ns = std::max<long long>(1, std::min<long long>(num_cu / p->nqt, tiles));
         p->rows_per_slice = (tiles + ns - 1) / ns * 256;
         p->nslices = (int)((nrows + p->rows_per_slice - 1) / p->rows_per_slice);
@@ -889,6 +893,8 @@ hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& 
     P.gtop = p.gtop_m ? P.gthr + (size_t)p.nqt * p.tq : nullptr;
     P.gtop_m = p.gtop_m;
     P.fold_mask = P.gtop ? 0x11111111u : 0x55555555u;   // scheduled folds after row tiles 1, 16, 256, ... (1, 4, 16, ... without the bound)
+    // (where first thresholds are there and two tiles follow at most, the first fold costs more than it saves: 100000 x 4096, 64 queries 201 us, 179 without)
+    if (p.kp <= 64 && p.rows_per_slice <= 3 * 256) P.fold_mask &= ~1u;
     const size_t words = p.share_bytes / sizeof(unsigned);
     hipLaunchKernelGGL(f8_zero_kernel, dim3((unsigned)std::min<size_t>((words + 255) / 256, 4096)), dim3(256), 0, s, P.gthr, words);
     switch (p.r) {

@@ -452,14 +452,15 @@ def test_product_in_every_tile(ssa, m, n, k):
 
 
 @pytest.mark.parametrize("n,d,nq,k", [(70000, 130, 129, 10), (140000, 64, 300, 49), (66000, 200, 700, 100), (40000, 128, 1025, 1), (513, 400, 200, 48), (20000, 1100, 150, 300),
-                                      (70000, 64, 100, 10), (70000, 520, 20, 30)])
+                                      (70000, 64, 100, 10), (70000, 520, 20, 30),
+                                      (140000, 64, 520, 10), (140000, 300, 400, 60), (128 * 1024 + 1, 130, 500, 48), (10000, 768, 900, 10)])
 def test_search_of_large_batches_over_many_row_tiles(ssa, n, d, nq, k):
     X, Q = unit_rows(n, d, SALT + n + d), unit_rows(nq, d, SALT + nq)
     index = filled(ssa, cuda(X))
     check_search(*index.search(Q, k), plain.round_rows(X), plain.round_rows(Q), k)
 
 
-@pytest.mark.parametrize("nq", [20, 100, 300])
+@pytest.mark.parametrize("nq", [20, 100, 300, 800])
 @pytest.mark.parametrize("k", [10, 60])
 def test_search_of_rows_that_get_better_and_better(ssa, nq, k):
     """Every row tile beats all before it: each threshold is late.  The values are exact, with many equal ones."""
@@ -480,11 +481,14 @@ def test_large_batches_over_many_segments(ssa, monkeypatch):
     index = filled(ssa, X)
     for nq in (16, 128, 310):
         check_search(*index.search(Q[:nq], 12), plain.round_rows(X), plain.round_rows(Q[:nq]), 12)
+    monkeypatch.setenv("SSMI_SEG_SHIFT", "11")
+    X, Q = unit_rows(120000, 64, SALT + 24), unit_rows(560, 64, SALT + 25)
+    check_search(*filled(ssa, X).search(Q, 12), plain.round_rows(X), plain.round_rows(Q), 12)
 
 
-@pytest.mark.parametrize("nq", [12, 100, 300])
-def test_large_batches_of_rows_and_queries_that_are_not_finite(ssa, nq):
-    X, Q = unit_rows(3000, 256, SALT + 22), unit_rows(nq, 256, SALT + 23)
+@pytest.mark.parametrize("n,nq", [(3000, 12), (3000, 100), (3000, 300), (130000, 520)])
+def test_large_batches_of_rows_and_queries_that_are_not_finite(ssa, n, nq):
+    X, Q = unit_rows(n, 256, SALT + 22), unit_rows(nq, 256, SALT + 23)
     X[::2, 7] = np.nan    # half the rows of every tile
     X[1:600:2, 200] = np.inf
     Q[3, 0] = np.nan
