@@ -45,6 +45,7 @@ struct F8NormArgs {
     void* residual_out; long long ro_stride;
     const void* weight; int weight_dtype;              // nullptr: none
     float eps;
+    double inv_d;                                      // 1 / d
     bool norm, unit;
     long long n;
     int d, dtype;

@@ -252,6 +252,7 @@ int ssmi_f8_rms_norm(int device, int64_t n, int d, const void* x, int dtype, int
     a.weight = weight;
     a.weight_dtype = weight_dtype;
     a.eps = eps;
+    a.inv_d = 1.0 / d;
     a.norm = true;
     a.unit = unit != 0;
     HIPCHECK(launch_f8_rows(a, cus, (hipStream_t)stream));

@@ -74,9 +74,12 @@ __device__ __forceinline__ void row_sums(double& a, double& b, double2* lds) {
 // The norm's sums and its one factor per row are 64-bit: y is then the exact value rounded once, and an element's code is that of
 // the exact row unless y lies within 2^-24 of a border.  (With fp32 sums and factors three times as many codes parted from the exact
 // ones; the 64-bit products hide behind memory.)  unit needs no second pass: |y| = f |h w| for y = f h w.
+// The quantiser is bound by memory (200000 x 2048 fp32: 376 us, 5.4 TB/s), the norm by what little of its rows is in flight while it
+// reduces (32768 x 4096 bf16 with a residual: 238 us, 4.0 TB/s; 200000 x 2048 fp32, unit: 445 us, 4.6 TB/s; a row of 4096 per wave
+// needs 254 registers and took 574 us).
 // (Four passes of 1024 threads would take rows of 32768 elements through the norm, but spill.)
 template <typename T, int ITER, bool WAVE, bool VEC, bool NORM>
-__global__ void __launch_bounds__(WAVE ? 256 : 1024) f8_rows_kernel(F8NormArgs a) {
+__global__ void __launch_bounds__(WAVE ? 256 : 1024, WAVE ? 1 : 5) f8_rows_kernel(F8NormArgs a) {
     __shared__ double2 red[16];
     const int tpr = WAVE ? 64 : (int)blockDim.x;
     const int t = WAVE ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
@@ -130,8 +133,9 @@ __global__ void __launch_bounds__(WAVE ? 256 : 1024) f8_rows_kernel(F8NormArgs a
                     }
                 }
                 row_sums<WAVE>(hh, yy, red);
-                double f = 1.0 / sqrt(hh / (double)a.d + (double)a.eps);
-                if (a.unit) f /= fmax(f * sqrt(yy), 1e-12);
+                // (every lane computes the factor: a 64-bit root and division each took as long as the row's own arithmetic)
+                double f = rsqrt(fma(hh, a.inv_d, (double)a.eps));
+                if (a.unit) f = yy * f * f >= 1e-24 ? rsqrt(yy) : f * 1e12;   // |y| = f sqrt(yy), below 1e-12 the divisor stays there
 #pragma unroll
                 for (int i = 0; i < ITER; ++i) {
                     float w[8];
