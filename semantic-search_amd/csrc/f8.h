@@ -4,8 +4,8 @@
 //
 // codes: OCP e4m3 (largest finite value 448, no infinity, 0x7f / 0xff = NaN), rows padded with zero codes to whole blocks.
 // b: E8M0 exponent bytes, 255 = NaN.  The quantiser takes the smallest power of two s with max|x| <= 448 s and rounds x / s
-// to nearest even.  Powers of two, for two reasons: v_mfma_scale_f32_16x16x128_f8f6f4 takes one E8M0 byte per operand row and
-// block of K = 128 and applies it for nothing, and quantising the values of a quantised row gives the same values (a block
+// to nearest even.  Powers of two, for two reasons: a value still has four significant bits, so that bf16 holds it and the matrix
+// cores take it exactly (f8_tile.h), and quantising the values of a quantised row gives the same values (a block
 // whose largest code rounded down to 224 halves its scale and doubles its codes).
 #pragma once
 #include "kernels.h"

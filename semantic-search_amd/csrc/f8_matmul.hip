@@ -2,8 +2,8 @@
 //
 //   out[i][j] = sum over blocks b of 2^(sa[i,b] - 127) 2^(sb[j,b] - 127) sum over the 128 codes of b of a[i,.] b[j,.]
 //
-// rounded once to 16 bits.  Tiles of 256 x 256 with a wave per SIMD where they fill the chip, tiles of 128 x 128 and 64 x 64 below
-// that, and where those would leave most CUs idle (a decoding batch) smaller ones whose waves share K.
+// exact products summed in fp32 (f8_tile.h), rounded once to 16 bits.  Tiles of 256 x 256 with a wave per SIMD where they fill the chip, tiles
+// of 128 x 128 and 64 x 64 below that, and where those would leave most CUs idle (a decoding batch) smaller ones whose waves share K.
 #include <algorithm>
 #include <initializer_list>
 #include "f8_big.h"
@@ -97,10 +97,7 @@ __global__ void __launch_bounds__(WM * WN * 64) f8_matmul_tile_kernel(F8MatmulAr
     F8Src x{p.b.codes + j0 * p.b.stride, p.b.scales + j0 * p.b.sstride, (unsigned)p.b.stride, (unsigned)p.b.sstride, (int)min((long long)T::XR - 1, p.b.n - 1 - j0)};
     F8Src q{p.a.codes + i0 * p.a.stride, p.a.scales + i0 * p.a.sstride, (unsigned)p.a.stride, (unsigned)p.a.sstride, (int)min((long long)T::QR - 1, p.a.n - 1 - i0)};
     f32x4_t acc[MT][NT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    zero_acc(acc);
     T t;
     t.init(smem, p.nblk);
     t.aim(x, q);
@@ -117,8 +114,8 @@ __global__ void __launch_bounds__(WM * WN * 64) f8_matmul_tile_kernel(F8MatmulAr
 // 256 x 256 tiles, a wave per SIMD: workgroups stay, the first slab of the next tile travels under this one's epilogue.
 // Tiles are numbered in bands of eight along a, and consecutive workgroups go round the XCDs: the 32 tiles of an XCD cover 8 x 4,
 // twelve operand panels for its L2.
-// 8192^3: 455 us, 2.42 PFLOP/s; 4096 x 8192 x 8192: 198 us, 2.78; 4096^3: 61 us, 2.24 (8192^3 in tiles of 128 x 128: 585 us).
-// The matrix pipe alone reaches 4.9 PFLOP/s on registers, with the operands' way through LDS the chip's power is the limit.
+// 8192^3: 694 us, 1.58 PFLOP/s; 4096 x 8192 x 8192: 357 us, 1.54; 4096^3: 97 us, 1.41 (8192^3 in tiles of 128 x 128: 878 us).  The bf16
+// instruction alone reaches 1.75 PFLOP/s on registers: the chip's power is the limit, and codes in LDS take half the bytes of bf16 there.
 template <bool BF>
 __global__ void __launch_bounds__(256, 1) f8_matmul_big_kernel(F8MatmulArgs p) {
     extern __shared__ __align__(16) unsigned char smem[];
@@ -137,12 +134,7 @@ __global__ void __launch_bounds__(256, 1) f8_matmul_big_kernel(F8MatmulArgs p) {
     if (logical < tiles) aim(logical);
     for (int tile = logical; tile < tiles; tile += gridDim.x) {
         F8Big::Acc acc;
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
+        zero_acc(acc);
         t.run(acc);
         const int lane = F8Big::lane_now();
         const F8Out o = out_tile(p, i0, j0);
@@ -159,7 +151,7 @@ __global__ void __launch_bounds__(256, 1) f8_matmul_big_kernel(F8MatmulArgs p) {
 }
 
 // Few rows of a: (16 NT) rows of a x (16 MT) rows of b per workgroup.  Its W waves share K, each with a ring of its own and no
-// barrier, and add up through LDS.  1 x 4096 x 4096: 5.0 us; 64 x 4096 x 4096: 5.8 us, 2.9 TB/s of b; 128 x 4096 x 4096: 6.8 us.
+// barrier, and add up through LDS.  1 x 4096 x 4096: 6.0 us; 64 x 4096 x 4096: 6.4 us, 2.6 TB/s of b; 128 x 4096 x 4096: 8.5 us.
 template <int MT, int NT, int W, int S, bool BF>
 __global__ void __launch_bounds__(W * 64) f8_matmul_split_kernel(F8MatmulArgs p) {
     using T = F8Tile<MT, NT, 1, 1, S, true>;
@@ -170,10 +162,7 @@ __global__ void __launch_bounds__(W * 64) f8_matmul_split_kernel(F8MatmulArgs p)
     const int each = ((p.nblk + W - 1) / W + 3) & ~3;   // whole scale words
     const int kb = wave * each, nblk = min(each, p.nblk - kb);
     f32x4_t acc[MT][NT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    zero_acc(acc);
     T t;
     t.init(smem + wave * T::LDS, nblk);
     if (nblk > 0) {
@@ -233,33 +222,40 @@ static hipError_t launch_split(F8MatmulArgs& p, hipStream_t s) {
 }
 template <bool BF>
 static hipError_t launch_t(F8MatmulArgs& p, int num_cu, hipStream_t s) {
-    const long long m = p.a.n, n = p.b.n;
-    const long long nb = p.nblk, t64 = ((m + 63) / 64) * ((n + 63) / 64);
-    // One launch of T tiles takes as many rounds as it has times the chip's places for their workgroups.  A round's time was
-    // measured as (fixed part) + (part per block of K), in units of 10 ns, e.g. 33.8 us for 2048 x 4096 x 4096 in tiles of 128 x 128.
+    // One launch of T tiles takes as many rounds as it has times the chip's places for their workgroups.  A round's time was measured as
+    // (fixed part) + (part per block of K), in units of 10 ns, for 1 to 8192 rows of a, 700 to 32768 of b and K of 141 to 8192; the least is within
+    // a tenth of the fastest tile for 33 of 35 sizes.  All tiles read slabs at the rate of the caches and convert every fragment that a wave
+    // multiplies, so that small tiles cost less per tile and more per product.  us in tiles of (a x b) 16 x 16, 32 x 32, 64 x 32, 64 x 64 whose waves
+    // share K, and of 64 x 64, 128 x 128 and 256 x 256 whose waves share slabs, K = 4096:
+    //     1 x 4096      6.6    6.0    8.1   10.8    14.4   31.1   65.5
+    //    64 x 4096     11.6    6.4    8.5   11.0    15.1   32.1   65.3
+    //   128 x 4096     21.2   10.1    8.5   11.2    14.8   32.8   66.3
+    //   256 x 4096     41.3   18.3   15.1   11.8    15.4   32.7   67.5
+    //    16 x 12288    11.7   11.4   14.8   12.1    14.7   31.5   66.1
+    //    48 x 12288    24.6   14.6   15.1   12.2    14.9   32.1   66.2
+    //   512 x 4096     82.4   35.1   28.4   21.6    22.5   33.0   67.6
+    //  1024 x 4096      169   74.6   57.0   42.7    42.5   34.2   67.6
+    //  2048 x 4096        -      -    149   93.3    89.5   57.7   72.2
+    //  4096 x 4096        -      -    288    178     177    121   97.3
+    // and K = 1024: 512 x 4096 in 64 x 64 8.7 (12.7 with shared K, 11.7 in 128 x 128), 1024 x 4096 14.9 (23.7, 12.5).
+    const long long m = p.a.n, n = p.b.n, nb = p.nblk;
+    const auto tiles = [&](int tm, int tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); };
     const auto cost = [&](int tm, int tn, int places, long long fixed, long long block) {
-        const long long tiles = ((m + tm - 1) / tm) * ((n + tn - 1) / tn), at_once = (long long)places * num_cu;
-        return (tiles + at_once - 1) / at_once * (fixed + block * nb);
+        const long long at_once = (long long)places * num_cu;
+        return (tiles(tm, tn) + at_once - 1) / at_once * (fixed + block * nb);
     };
-    const auto least = [](std::initializer_list<long long> c) { return std::min_element(c.begin(), c.end()) - c.begin(); };
-    // A workgroup gets 57 B/ns from the caches at best, so where tiles are few the waves share K and the tiles are small (us in tiles
-    // of 32 x 32, 64 x 32 and 64 x 64, and of 64 x 64 whose waves share slabs: 64 x 4096 x 4096 5.8, 6.5, 8.0, 9.7; 128 x 4096 x 4096 8.7, 6.8, 7.9,
-    // 10.2; 1 x 4096 x 4096 in 16 x 16 5.0, else 6.0).  With more tiles than CUs slabs that are shared win (512 x 4096 x 4096 23.2 in 64 x 32, 15.7), and
-    // for few rows of a already where the tiles fill most of the chip: b then streams from memory (16 x 12288 x 4096 12.1, 10.0)
-    if (t64 <= num_cu && (m > 64 || 4 * t64 < 3 * num_cu)) {
-        switch (least({cost(16, 16, 1, 80, 7), cost(32, 32, 1, 70, 12), cost(64, 32, 1, 190, 14), cost(64, 64, 1, 250, 19)})) {
-            case 0: return launch_split<1, 1, 8, 3, BF>(p, s);
-            case 1: return launch_split<2, 2, 8, 2, BF>(p, s);
-            case 2: return launch_split<2, 4, 4, 3, BF>(p, s);
-            default: return launch_split<4, 4, 4, 2, BF>(p, s);
-        }
-    }
-    // (tiles of 64 x 64, 128 x 128 of one workgroup per CU and of two, 256 x 256: 512 x 4096 x 4096 15.7, 19.9, 25.5, 40.0;
-    // 1024 x 4096 x 4096 30.6, 22.4, 28.4, 41.4; 2048 x 4096 x 4096 72.6, 43.3, 35.5, 43.3; 4096^3 149, 94, 72, 56)
-    switch (least({t64 <= num_cu ? 200 + 25 * nb : cost(64, 64, 2, 200, 36), cost(128, 128, 1, 330, 55), cost(128, 128, 2, 500, 90), cost(256, 256, 1, 650, 166)})) {
-        case 0: return launch_tile<2, 2, 2, 2, 4, BF>(p, s);
-        case 1: return launch_tile<4, 2, 2, 4, 4, BF>(p, s);
-        case 2: return launch_tile<4, 4, 2, 2, 2, BF>(p, s);
+    // (two workgroups of a CU share its caches and pipes: alone each is faster)
+    const std::initializer_list<long long> us = {
+        cost(16, 16, 1, 160, 6), cost(32, 32, 1, 240, 6), cost(64, 32, 1, 300, 13), cost(64, 64, 1, 430, 20),
+        tiles(64, 64) <= num_cu ? 340 + 34 * nb : cost(64, 64, 2, 240, 60), tiles(128, 128) <= num_cu ? 260 + 90 * nb : cost(128, 128, 2, 460, 173),
+        cost(256, 256, 1, 1400, 255)};
+    switch (std::min_element(us.begin(), us.end()) - us.begin()) {
+        case 0: return launch_split<1, 1, 8, 3, BF>(p, s);
+        case 1: return launch_split<2, 2, 8, 2, BF>(p, s);
+        case 2: return launch_split<2, 4, 4, 3, BF>(p, s);
+        case 3: return launch_split<4, 4, 4, 2, BF>(p, s);
+        case 4: return launch_tile<2, 2, 2, 2, 4, BF>(p, s);
+        case 5: return launch_tile<4, 4, 2, 2, 2, BF>(p, s);
         default: return launch_big<BF>(p, num_cu, s);
     }
 }

@@ -1,15 +1,15 @@
 // f8_pp.h - the contraction of f8_tile.h for tiles of 256 rows x 256 queries, scheduled so that the matrix pipe of every SIMD
-// is fed without a pause (the schedule of the 16-bit kernel, mfma_pp.hip, with 128-code slabs).  A product of 8192^3 took 484 us on it and
-// 455 us on f8_big.h; but there the accumulators fill half the registers of a wave that is alone on its SIMD, and a search's filter spills.
+// is fed without a pause (the schedule of the 16-bit kernel, mfma_pp.hip, with 128-code slabs).  f8_big.h reads and converts less, but there the
+// accumulators fill half the registers of a wave that is alone on its SIMD, and a search's filter spills.
 //
 // Eight waves = two groups of four (group g = waves 4g..4g+3, one wave of each group per SIMD), wave tile 128 rows x 64 queries =
-// 4 x 2 accumulators of v_mfma_scale_f32_32x32x64_f8f6f4.  K is walked in PHASES of 64 codes, the operands arrive in slabs of
+// 4 x 2 accumulators of v_mfma_f32_32x32x16_bf16.  K is walked in PHASES of 64 codes, the operands arrive in slabs of
 // 128 (one scale block; 256 rows x 128 B = 32 KiB each) in a ring of two.
 //
 //   LOAD(p)   p even: issue the eight 1 KiB pieces of slab p/2 + 1; ds_read the fragments of phase p
 //             p odd, group 1: s_waitcnt vmcnt(0)
 //             s_barrier
-//   MFMA(p)   eight MFMAs
+//   MFMA(p)   32 MFMAs, and under them the fragments become operands
 //             p odd, group 0: s_waitcnt vmcnt(0)
 //             s_barrier
 //
@@ -36,7 +36,8 @@ struct F8Pp {
     unsigned char* smem;
     int lane, wave, wm, wn, nblk;
     const unsigned char *xc, *qc, *sc;                    // codes of the tiles; scales of the operand this wave brings
-    unsigned xo[4], qo[4], so;
+    unsigned xstride, qstride, so;
+    int xlast, qlast;
 
     __device__ __forceinline__ void init(unsigned char* lds, int blocks) {
         smem = lds;
@@ -48,13 +49,10 @@ struct F8Pp {
     }
     // sources of a tile; starts its pipeline (slab 0 and the first scale words).  No wave may still read the ring
     __device__ __forceinline__ void aim(const F8Src& x, const F8Src& q) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = (wave * 4 + j) * 8 + (lane >> 3);
-            const unsigned c = ((lane & 7) ^ ((r >> 1) & 7)) * 16;
-            xo[j] = (unsigned)min(r, x.last) * x.stride + c;
-            qo[j] = (unsigned)min(r, q.last) * q.stride + c;
-        }
+        xstride = x.stride;
+        qstride = q.stride;
+        xlast = x.last;
+        qlast = q.last;
         xc = x.codes;
         qc = q.codes;
         const int r = (wave & 3) * 64 + lane;
@@ -68,9 +66,15 @@ struct F8Pp {
         // (uniform addresses that the compiler may not fold with the lanes' offsets: it would keep the 64-bit sums in registers)
         const unsigned char *xb = xc + (size_t)d * 128, *qb = qc + (size_t)d * 128;
         asm volatile("" : "+s"(xb), "+s"(qb));
+        // (offsets made anew for every piece: chunk c of row r0 + 8 j; kept in registers, the search's filter spilled.  Rows < 256 and strides of
+        // at most 2^23 bytes: 24 bits)
+        int l = lane;
+        asm volatile("" : "+v"(l));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            unsigned o = j < 4 ? xo[j & 3] : qo[j & 3];
+            const int r = wave * 32 + (j & 3) * 8 + (l >> 3);
+            const unsigned chunk = ((l & 7) ^ ((l >> 4) + (j & 1) * 4)) * 16;   // (r >> 1) & 7
+            unsigned o = j < 4 ? __umul24((unsigned)min(r, xlast), xstride) + chunk : __umul24((unsigned)min(r, qlast), qstride) + chunk;
             asm volatile("" : "+v"(o));   // (a 32-bit offset, widened here and not ahead of the loop)
             if (j < 4) GLDS16(xb + o, dst + j * 1024);
             else GLDS16(qb + o, dst + 2 * SLAB + (j & 3) * 1024);
@@ -107,11 +111,16 @@ struct F8Pp {
             const unsigned char* cur = smem + (J & 1) * SLAB;   // (d & 1 == J & 1)
             i32x8_t a[4], b[2];
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
-                a[m] = join8(*reinterpret_cast<const i32x4_t*>(cur + a_row + m * 4096 + ch[2 * H]), *reinterpret_cast<const i32x4_t*>(cur + a_row + m * 4096 + ch[2 * H + 1]));
-#pragma unroll
             for (int n = 0; n < 2; ++n)
                 b[n] = join8(*reinterpret_cast<const i32x4_t*>(cur + b_row + n * 4096 + ch[2 * H]), *reinterpret_cast<const i32x4_t*>(cur + b_row + n * 4096 + ch[2 * H + 1]));
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                a[m] = join8(*reinterpret_cast<const i32x4_t*>(cur + a_row + m * 4096 + ch[2 * H]), *reinterpret_cast<const i32x4_t*>(cur + a_row + m * 4096 + ch[2 * H + 1]));
+            float fx[4], fq[2];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) fx[m] = f8_factor<J>(sx[m]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) fq[n] = f8_factor<J>(sq[n]);
             if (H == 1 && wm == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // fragments in registers
             __builtin_amdgcn_sched_barrier(0);
@@ -121,9 +130,18 @@ struct F8Pp {
             asm volatile("" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(b[0]), "+v"(b[1]));
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
+            for (int e = 0; e < 8; e += 2) {   // 16 codes of K; the conversions go under the products
+                i32x4_t bw[2];
 #pragma unroll
-                for (int n = 0; n < 2; ++n) acc[m][n] = mfma_f8_32<J>(a[m], b[n], acc[m][n], sx[m], sq[n]);
+                for (int n = 0; n < 2; ++n) bw[n] = f8_widen(b[n][e], b[n][e + 1], fq[n]);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const i32x4_t aw = f8_widen(a[m][e], a[m][e + 1], fx[m]);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) acc[m][n] = mfma_f8_32(aw, bw[n], acc[m][n]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             asm volatile("" : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1]), "+v"(acc[2][0]), "+v"(acc[2][1]), "+v"(acc[3][0]), "+v"(acc[3][1]));
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);

@@ -347,7 +347,13 @@ __global__ void __launch_bounds__(512) f8_scan_kernel(F8ScanArgs A) {
     for (int b = 0; b < BT; ++b) stage_query(A, min(b, nq - 1), qs + b * qpitch, qsc + b * spitch);
 
     f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const i32x4_t zero = i32x4_t{0, 0, 0, 0};
+    // a load of rows against the same codes of the queries: sixteen codes a lane, two instructions
+    const auto block = [&](auto jc, const i32x4_t& x, const i32x4_t& y, int sx, int sy) __attribute__((always_inline)) {
+        constexpr int J = decltype(jc)::value;
+        const float fx = f8_factor<J>(sx), fy = f8_factor<J>(sy);
+        acc = mfma_f8(f8_widen(x[0], x[1], fx), f8_widen(y[0], y[1], fy), acc);
+        acc = mfma_f8(f8_widen(x[2], x[3], fx), f8_widen(y[2], y[3], fy), acc);
+    };
     // a row group is complete: rows 4 ((lane >> 4) & 1) + i of it, even-even here, odd-odd in lane ^ 40
     auto offer = [&](int g) __attribute__((always_inline)) {
         float sum[4];
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(512) f8_scan_kernel(F8ScanArgs A) {
             const auto one = [&](auto jc) __attribute__((always_inline)) {
                 constexpr int J = decltype(jc)::value;
                 const i32x4_t y = *reinterpret_cast<const i32x4_t*>(qp + J * kF8Block);
-                acc = mfma_f8<J % 4>(join8(x[J], zero), join8(y, zero), acc, sc[J / 4], sq[J / 4]);
+                block(std::integral_constant<int, J % 4>(), x[J], y, sc[J / 4], sq[J / 4]);
             };
             const int left = nblk - ckb;   // (the rest of a row that is not whole stages)
             one(std::integral_constant<int, 0>());
@@ -397,10 +403,10 @@ __global__ void __launch_bounds__(512) f8_scan_kernel(F8ScanArgs A) {
             for (int j = 0; j < NB; ++j) y[j] = *reinterpret_cast<const i32x4_t*>(qlane + j * kF8Block);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                acc = mfma_f8<0>(join8(x[g * NB], zero), join8(y[0], zero), acc, sc[g], sq);
-                if constexpr (NB > 1) acc = mfma_f8<1>(join8(x[g * NB + 1], zero), join8(y[1], zero), acc, sc[g], sq);
-                if constexpr (NB > 2) acc = mfma_f8<2>(join8(x[g * NB + 2], zero), join8(y[2], zero), acc, sc[g], sq);
-                if constexpr (NB > 3) acc = mfma_f8<3>(join8(x[g * NB + 3], zero), join8(y[3], zero), acc, sc[g], sq);
+                block(std::integral_constant<int, 0>(), x[g * NB], y[0], sc[g], sq);
+                if constexpr (NB > 1) block(std::integral_constant<int, 1>(), x[g * NB + 1], y[1], sc[g], sq);
+                if constexpr (NB > 2) block(std::integral_constant<int, 2>(), x[g * NB + 2], y[2], sc[g], sq);
+                if constexpr (NB > 3) block(std::integral_constant<int, 3>(), x[g * NB + 3], y[3], sc[g], sq);
                 offer(g);
             }
         }
@@ -566,10 +572,7 @@ __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, 
     for (long long row0 = r_begin; row0 < r_end; row0 += 256) {
         const long long left = r_end - row0;
         f32x4_t acc[MT][NT];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        zero_acc(acc);
         t.run(acc);
         if (tiles_done == 0 && P.k <= 64) {
             float* maxima = reinterpret_cast<float*>(smem);   // (the ring is free)
@@ -702,12 +705,7 @@ __global__ void __launch_bounds__(512, 2) f8_search_big_kernel(F8View V, F8Mat q
 #pragma unroll 1
     for (long long row0 = r_begin; row0 < r_end; row0 += 256) {
         F8Pp::Acc acc;
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.f;
+        zero_acc(acc);
         t.run(acc);
         const long long left = r_end - row0;
         int lane = t.lane;

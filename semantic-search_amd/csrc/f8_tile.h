@@ -1,12 +1,15 @@
-// f8_tile.h - contraction of one tile of 8-bit rows with one tile of 8-bit queries on the scaled matrix instruction.
+// f8_tile.h - contraction of one tile of 8-bit rows with one tile of 8-bit queries on the matrix cores.
 //
 //   acc[row][query] = sum over blocks b of 2^(sx[row,b] - 127) 2^(sq[query,b] - 127) sum over the 128 codes of b of x q
 //
-// v_mfma_scale_f32_16x16x128_f8f6f4: K = 128 is one scale block, so the two E8M0 bytes of a (row, query) pair ride along with
-// the instruction (its operand selectors pick the byte of a word that holds four blocks) and no vector instruction touches
-// the products.  The instruction aligns the products of a block to the largest of them and drops what lies more than 13 bits
-// below it (measured: a sum over 4096 dimensions is off by 1.6e-5 of the scores' norm, where a chain of fp32 adds is off by
-// 5e-8): its sums are the candidates of a search, which scores them again in 64 bits, or leave rounded to 16 bits.
+// The operands travel as codes - a quarter of fp32 in memory, half of bf16 in LDS - and become bf16 on their way into the
+// instruction: v_cvt_scalef32_pk_bf16_fp8 takes two codes and the power of two of their block, four significant bits fit eight
+// (exact from 2^-133 to the end of fp32; scale byte 255 gives NaN), and at 4 cycles a pair it hides under v_mfma_f32_*_bf16.
+// Products of such operands are exact and the sums are fp32's: measured, an instruction is off by less than 2^-21.5 of the
+// magnitudes it adds, 2^-22 of an accumulator that is large beside them.
+// v_mfma_scale_f32_*_f8f6f4, which takes codes and scale bytes as they are at twice the rate (3.9 PFLOP/s on registers, 1.75), is not
+// used: it aligns the products of eight neighbouring codes to the largest of them and drops what lies more than 13 bits below
+// (measured; v_mfma_f32_*_fp8_fp8 does the same), so that a strong channel or two large products that cancel take the rest with them.
 #pragma once
 #include "f8.h"
 #include "mfma_common.h"
@@ -16,20 +19,36 @@ namespace ssmi {
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
+// byte J of a word of scales as the power of two it stands for, in the exponent of an fp32 (0 and 255 as f8_pair reads them)
 template <int J>
-__device__ __forceinline__ f32x4_t mfma_f8(const i32x8_t& a, const i32x8_t& b, const f32x4_t& c, int sa, int sb) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, J, sa, J, sb);
+__device__ __forceinline__ float f8_factor(int w) { return __int_as_float((int)(((unsigned)w >> (8 * J)) & 255u) << 23); }
+// codes 0, 1 (HI: 2, 3) of a word -> their values as bf16
+template <bool HI>
+__device__ __forceinline__ int f8_pair(int w, float s) {
+    return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)w, s, HI));
+}
+// eight codes of a lane -> an operand
+__device__ __forceinline__ i32x4_t f8_widen(int lo, int hi, float s) {
+    return i32x4_t{f8_pair<false>(lo, s), f8_pair<true>(lo, s), f8_pair<false>(hi, s), f8_pair<true>(hi, s)};
+}
+__device__ __forceinline__ f32x4_t mfma_f8(const i32x4_t& a, const i32x4_t& b, const f32x4_t& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16_t mfma_f8_32(const i32x4_t& a, const i32x4_t& b, const f32x16_t& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ i32x8_t join8(const i32x4_t& lo, const i32x4_t& hi) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-
-template <int J>
-__device__ __forceinline__ f32x16_t mfma_f8_32(const i32x8_t& a, const i32x8_t& b, const f32x16_t& c, int sa, int sb) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, J, sa, J, sb);
+// accumulators of whatever extent, zero
+template <typename V, int M, int N>
+__device__ __forceinline__ void zero_acc(V (&acc)[M][N]) {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[m][n] = V(0.f);
 }
 
 // One operand's tile: rows of a plain matrix or of one segment of a row store (uniform base, 32-bit offsets).
@@ -129,9 +148,9 @@ struct F8Tile {
 
     // the tile aimed at last; the ring is free (for the next aim) on return
     __device__ __forceinline__ void run(f32x4_t (&acc)[MT][NT]) {
-        const int frow = lane & 15, fq = lane >> 4;
+        const int frow = lane & 15, fgrp = lane >> 4;
         const int fsw = (frow >> 1) & 7;
-        const int c0 = (fq ^ fsw) * 16, c1 = ((4 + fq) ^ fsw) * 16;
+        const int c0 = (fgrp ^ fsw) * 16, c1 = ((4 + fgrp) ^ fsw) * 16;
         const int a_row = (wm * MT * 16 + frow) * 128, b_row = XR * 128 + (wn * NT * 16 + frow) * 128;
         int slot = 0, ahead = S - 1;
         int sx[MT], sq[NT];
@@ -160,10 +179,23 @@ struct F8Tile {
             __builtin_amdgcn_sched_barrier(0);   // (the reads in front of the pieces: the compiler would wait for pieces in flight in front of reads)
             if (d + S - 1 < nblk) slab(d + S - 1, ahead, ((J + S - 1) & 3) == 0);
             __builtin_amdgcn_sched_barrier(0);
+            float fx[MT], fq[NT];
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < MT; ++m) fx[m] = f8_factor<J>(sx[m]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) acc[m][n] = mfma_f8<J>(a[m], b[n], acc[m][n], sx[m], sq[n]);
+            for (int n = 0; n < NT; ++n) fq[n] = f8_factor<J>(sq[n]);
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {   // 32 codes of K
+                i32x4_t bw[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) bw[n] = f8_widen(b[n][e], b[n][e + 1], fq[n]);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const i32x4_t aw = f8_widen(a[m][e], a[m][e + 1], fx[m]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) acc[m][n] = mfma_f8(aw, bw[n], acc[m][n]);
+                }
+            }
             slot = slot == S - 1 ? 0 : slot + 1;
             ahead = ahead == S - 1 ? 0 : ahead + 1;
         };
