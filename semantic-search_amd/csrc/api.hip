@@ -56,12 +56,11 @@ int RowStore::init(int d_, int dtype_, hipStream_t stream) {
     return 0;
 }
 
-int RowStore::init_scales(const RowStore& codes, hipStream_t stream) {
-    d = f8_blocks(codes.d);
+int RowStore::init_side(const RowStore& codes, int bytes, hipStream_t stream) {
+    d = ld = bytes;
     dtype = codes.dtype;
     elsize = 1;
-    ld = (d + 15) / 16 * 16;
-    row_bytes = (size_t)ld;
+    row_bytes = (size_t)bytes;
     seg_shift = codes.seg_shift;
     HIPCHECK(hipMalloc((void**)&d_segs, sizeof(void*) * kMaxSegs));
     HIPCHECK(zero_device_sync(d_segs, sizeof(void*) * kMaxSegs, stream));
@@ -205,7 +204,12 @@ static int create_common(int d, int storage_dtype, int device, int kind, ssmi_in
     if (const char* e = getenv("SSMI_SHADOW_DTYPE")) h->shadow_pref = !strcmp(e, "f16") ? SSMI_F16 : (!strcmp(e, "bf16") ? SSMI_BF16 : -1);
     HIPCHECK(hipMalloc((void**)&h->d_flag, 256));
     CHECK(h->rows.init(d, storage_dtype, h->stream));
-    if (storage_dtype == SSMI_F8) CHECK(h->scales.init_scales(h->rows, h->stream));
+    if (storage_dtype == SSMI_F8) {
+        CHECK(h->scales.init_side(h->rows, (f8_blocks(d) + 15) / 16 * 16, h->stream));
+        CHECK(h->lengths.init_side(h->rows, sizeof(float), h->stream));
+        HIPCHECK(hipMalloc((void**)&h->f8_longest, 256));
+        HIPCHECK(zero_device_sync(h->f8_longest, 256, h->stream));
+    }
     guard.h = nullptr;
     *out = h;
     return 0;
@@ -265,6 +269,8 @@ int ssmi_index_free(ssmi_index* h) {
     ivf_destroy(h);
     h->rows.destroy();
     h->scales.destroy();
+    h->lengths.destroy();
+    if (h->f8_longest) (void)hipFree(h->f8_longest);
     if (h->has_shadow) h->shadow16.destroy();
     for (int i = 0; i < kWsSlots; ++i) if (h->ws[i]) (void)hipFree(h->ws[i]);
     if (h->tail_counters) (void)hipFree(h->tail_counters);
@@ -796,7 +802,7 @@ int ssmi_index_score_ids(ssmi_index* h, int64_t n, const int64_t* ids, int n_neg
     HIPCHECK(hipMemsetAsync(bad, 0, 4, h->stream));
     RowView v = R.view();
     if (h->kind == SSMI_KIND_IVFFLAT) v.nrows = h->ivf_slots_used;
-    if (R.dtype == SSMI_F8) HIPCHECK(launch_f8_score_rows(F8View{v, (const void* const*)h->scales.d_segs, h->scales.ld}, dids, n, R.d, dneg, n_neg, dout, bad, h->stream));
+    if (R.dtype == SSMI_F8) HIPCHECK(launch_f8_score_rows(F8View{v, (const void* const*)h->scales.d_segs, h->scales.ld, nullptr}, dids, n, R.d, dneg, n_neg, dout, bad, h->stream));
     else HIPCHECK(launch_score_rows(v, R.dtype, dids, n, R.d, dneg, n_neg, dout, bad, h->stream));
     HIPCHECK(hipMemcpyAsync(out_host, dout, (size_t)n * n_neg * 4, hipMemcpyDeviceToHost, h->stream));
     HIPCHECK(hipStreamSynchronize(h->stream));

@@ -18,6 +18,7 @@ namespace ssmi {
 static constexpr int kF8 = 3;             // SSMI_F8
 static constexpr int kF8Block = 128;      // codes per scale
 static constexpr int kF8Spare = 16;       // candidates beyond k that a search scores again in 64 bits
+static constexpr int kF8Batch = 4096;     // queries of a search that travel together
 static constexpr int kF8MaxNorm = 16384;  // elements of a row that the norm keeps in registers
 static constexpr int kF8MaxK = kMaxK - kF8Spare;
 
@@ -37,6 +38,7 @@ struct F8View {
     RowView X;                // ld = codes per row
     const void* const* ssegs;
     int sld;                  // scale bytes per row (multiple of 16)
+    const void* const* lsegs; // lengths, a float a row
 };
 
 struct F8NormArgs {
@@ -61,6 +63,14 @@ hipError_t launch_f8_score_rows(const F8View& v, const int64_t* ids, long long n
                                 int* bad, hipStream_t s);
 // out[i][j] = <a_i, b_j>, (a.n, b.n) of out_dtype (SSMI_F16 / SSMI_BF16), row stride in elements
 hipError_t launch_f8_matmul(const F8Mat& a, const F8Mat& b, int k, void* out, int out_dtype, long long out_stride, int num_cu, hipStream_t s);
+
+// the lengths of rows, rounded up (a row that holds a NaN: -1), and *longest (the bits of a positive float) = the largest of it and them
+hipError_t launch_f8_lengths(const F8Mat& m, int ld, float* lengths, unsigned* longest, int num_cu, hipStream_t s);
+
+// What the second pass of a search leaves for the third.  ticket 0: the query is answered; else it counts the workgroups that are done with it,
+// from 1, and pos their entries.  No row with a score below edge is among the k best, nor one that is not on the list and shorter than `from`.
+struct F8State { double edge; float from; unsigned ticket, pos, unused; };
+struct F8Entry { double score; long long id; };
 
 // search over a row store: the k best of every query with their scores summed in 64 bits
 struct F8SearchPlan {
@@ -93,9 +103,14 @@ struct F8ScanArgs {
     int64_t id_offset;
     unsigned min_ord;
     int cap, every;
+    const float* longest;     // no row is longer
+    F8State* state;           // [q.n], written by the second pass
+    F8Entry* lists;           // [num_cu][k], of the exact pass
 };
 hipError_t launch_f8_scan(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s);
 hipError_t launch_f8_finish(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s);
+// the queries whose lists the second pass could not prove, over all rows in 64 bits
+hipError_t launch_f8_exact(const F8ScanArgs& a, int num_cu, hipStream_t s);
 
 #ifdef __HIPCC__
 // two e4m3 codes per call from the low or high half of a word

@@ -44,14 +44,15 @@ int num_cu_of(int device, int* out) {
     return 0;
 }
 
-// rows of the handle's two stores that share a segment: f(first row of the run within the call, count, codes, scales)
+// rows of the handle's two stores that share a segment: f(first row of the run within the call, count, codes, scales, lengths)
 template <typename F>
 int for_segments(ssmi_index* h, long long row0, long long n, F f) {
     const long long seg_rows = 1ll << h->rows.seg_shift;
     for (long long done = 0; done < n;) {
         const long long row = row0 + done, seg = row >> h->rows.seg_shift, off = row & (seg_rows - 1);
         const long long cnt = std::min(n - done, seg_rows - off);
-        CHECK(f(done, cnt, (unsigned char*)h->rows.segs[seg] + off * h->rows.row_bytes, (unsigned char*)h->scales.segs[seg] + off * h->scales.row_bytes));
+        CHECK(f(done, cnt, (unsigned char*)h->rows.segs[seg] + off * h->rows.row_bytes, (unsigned char*)h->scales.segs[seg] + off * h->scales.row_bytes,
+                (float*)h->lengths.segs[seg] + off));
         done += cnt;
     }
     return 0;
@@ -59,7 +60,8 @@ int for_segments(ssmi_index* h, long long row0, long long n, F f) {
 int reserve_rows(ssmi_index* h, int64_t n) {
     if ((unsigned long long)(h->rows.nrows + n) >= 0xFFFFFFFFull) return fail("index would exceed 2^32-2 vectors");
     CHECK(h->rows.reserve(h->rows.nrows + n, h->stream));
-    return h->scales.reserve(h->rows.nrows + n, h->stream);
+    CHECK(h->scales.reserve(h->rows.nrows + n, h->stream));
+    return h->lengths.reserve(h->rows.nrows + n, h->stream);
 }
 F8NormArgs plain_rows(const void* x, int64_t x_stride, int dtype, int64_t n, int d, unsigned char* codes, int64_t stride,
                       unsigned char* scales, int64_t sstride) {
@@ -78,9 +80,10 @@ F8NormArgs plain_rows(const void* x, int64_t x_stride, int dtype, int64_t n, int
 // rows on the device -> the stores' rows [row0, row0 + n), which are reserved
 int quantize_into(ssmi_index* h, const void* x, int src_dtype, long long row0, long long n) {
     const int d = h->rows.d;
-    return for_segments(h, row0, n, [&](long long first, long long cnt, unsigned char* codes, unsigned char* scales) -> int {
+    return for_segments(h, row0, n, [&](long long first, long long cnt, unsigned char* codes, unsigned char* scales, float* lengths) -> int {
         HIPCHECK(launch_f8_rows(plain_rows((const char*)x + (size_t)first * d * dtype_elsize(src_dtype), d, src_dtype, cnt, d, codes, h->rows.ld, scales, h->scales.ld),
                                 h->num_cu, h->stream));
+        HIPCHECK(launch_f8_lengths(F8Mat{codes, h->rows.ld, scales, h->scales.ld, cnt}, h->rows.ld, lengths, (unsigned*)h->f8_longest, h->num_cu, h->stream));
         return 0;
     });
 }
@@ -106,7 +109,7 @@ int f8_store_add(ssmi_index* h, int64_t n, const void* x, int src_dtype, int mem
         if (mem_kind == SSMI_HOST) HIPCHECK(hipStreamSynchronize(h->stream));  // staging buffer reused
     }
     HIPCHECK(hipStreamSynchronize(h->stream));
-    h->rows.nrows = h->scales.nrows = row0 + n;
+    h->rows.nrows = h->scales.nrows = h->lengths.nrows = row0 + n;
     return 0;
 }
 
@@ -122,7 +125,7 @@ int f8_add_random_unit(ssmi_index* h, int64_t n, uint64_t seed) {
         CHECK(quantize_into(h, h->ws[0], SSMI_F32, row0 + done, cnt));
     }
     HIPCHECK(hipStreamSynchronize(h->stream));
-    h->rows.nrows = h->scales.nrows = row0 + n;
+    h->rows.nrows = h->scales.nrows = h->lengths.nrows = row0 + n;
     return 0;
 }
 
@@ -130,17 +133,17 @@ hipError_t gather_store_rows(ssmi_index* h, const RowStore& R, long long view_ro
                              hipStream_t s) {
     RowView v = R.view();
     v.nrows = view_rows;
-    if (R.dtype == SSMI_F8) return launch_f8_gather(F8View{v, (const void* const*)h->scales.d_segs, h->scales.ld}, ids, n, R.d, out, bad, s);
+    if (R.dtype == SSMI_F8) return launch_f8_gather(F8View{v, (const void* const*)h->scales.d_segs, h->scales.ld, nullptr}, ids, n, R.d, out, bad, s);
     return launch_gather_rows(v, R.dtype, ids, n, R.d, out, bad, s);
 }
 
-// Workspaces: 4 query codes and scales, 5 candidate buffers, 2 partial lists, 7 shared thresholds.
+// Workspaces: 4 query codes and scales, 5 candidate buffers, 2 partial lists, 6 states and lists of the exact pass, 7 shared thresholds.
 int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float* Ddev, int64_t* Idev, int64_t id_offset, hipStream_t s,
                     unsigned min_ord) {
     const RowStore& R = h->rows;
     const int ld = R.ld, sld = h->scales.ld;
-    const F8View view{R.view(), (const void* const*)h->scales.d_segs, sld};
-    const int64_t kBatch = 4096;
+    const F8View view{R.view(), (const void* const*)h->scales.d_segs, sld, (const void* const*)h->lengths.d_segs};
+    const int64_t kBatch = kF8Batch;
     hipEvent_t* ev = h->ev[h->n_searches % ssmi_index::kEvRing];
     F8SearchPlan p = {};
     for (int64_t done = 0; done < nq; done += kBatch) {
@@ -148,6 +151,7 @@ int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float*
         if (!plan_f8_search(ld, R.nrows, nb, k, h->num_cu, &p)) return fail("internal: 8-bit search plan failed");
         const bool rec = h->timing_on && done == 0;
         CHECK(ensure_ws(h, 2, p.partial_bytes));
+        CHECK(ensure_ws(h, 6, (size_t)nb * sizeof(F8State) + (size_t)h->num_cu * k * sizeof(F8Entry)));
         F8ScanArgs a = {};
         a.v = view;
         a.q = F8Mat{q.codes + done * q.stride, q.stride, q.scales + done * q.sstride, q.sstride, nb};
@@ -164,6 +168,9 @@ int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float*
         a.min_ord = min_ord;
         a.cap = p.cap;
         a.every = p.every;
+        a.longest = h->f8_longest;
+        a.state = (F8State*)h->ws[6];
+        a.lists = (F8Entry*)(a.state + nb);
         if (p.scan) {
             if (h->tail_counters) {
                 a.counter = nb == 1 ? h->tail_counters : nullptr;
@@ -171,8 +178,7 @@ int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float*
             }
             if (rec) HIPCHECK(hipEventRecord(ev[0], s));
             HIPCHECK(launch_f8_scan(a, p, s));
-            if (rec) { HIPCHECK(hipEventRecord(ev[1], s)); h->merge_event = false; }
-            if (a.counter) continue;
+            if (rec) HIPCHECK(hipEventRecord(ev[1], s));
         } else {
             if (q.f32) {
                 const size_t codes = (size_t)nb * ld;
@@ -188,7 +194,8 @@ int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float*
             HIPCHECK(launch_f8_tiles(view, a.q, p, h->ws[7], h->ws[5], (skey_t*)h->ws[2], s));
             if (rec) HIPCHECK(hipEventRecord(ev[1], s));
         }
-        HIPCHECK(launch_f8_finish(a, p, s));
+        if (!a.counter) HIPCHECK(launch_f8_finish(a, p, s));
+        HIPCHECK(launch_f8_exact(a, h->num_cu, s));
         if (rec) { HIPCHECK(hipEventRecord(ev[2], s)); h->merge_event = true; }
     }
     if (h->timing_on) h->n_searches++;
@@ -308,14 +315,15 @@ int ssmi_index_add_f8(ssmi_index* h, int64_t n, const uint8_t* codes, int64_t co
     quiesce(h);
     CHECK(reserve_rows(h, n));
     const int ns = f8_blocks(h->rows.d);
-    CHECK(for_segments(h, h->rows.nrows, n, [&](long long first, long long cnt, unsigned char* c, unsigned char* s) -> int {
+    CHECK(for_segments(h, h->rows.nrows, n, [&](long long first, long long cnt, unsigned char* c, unsigned char* s, float* lengths) -> int {
         HIPCHECK(hipMemcpy2DAsync(c, h->rows.ld, codes + first * codes_stride, codes_stride, h->rows.ld, cnt, hipMemcpyDeviceToDevice, h->stream));
         HIPCHECK(hipMemcpy2DAsync(s, h->scales.ld, scales + first * scales_stride, scales_stride, ns, cnt, hipMemcpyDeviceToDevice, h->stream));
+        HIPCHECK(launch_f8_lengths(F8Mat{c, h->rows.ld, s, h->scales.ld, cnt}, h->rows.ld, lengths, (unsigned*)h->f8_longest, h->num_cu, h->stream));
         return 0;
     }));
     HIPCHECK(hipStreamSynchronize(h->stream));
     h->rows.nrows += n;
-    h->scales.nrows = h->rows.nrows;
+    h->scales.nrows = h->lengths.nrows = h->rows.nrows;
     return 0;
     });
 }

@@ -1,10 +1,14 @@
 // f8_search.hip - Flat search over 8-bit rows (f8.h): the product of f8_tile.h with the top-k epilogues of the other row types.
 //
-// Two passes.  The first keeps, for every query, the best k + 16 rows by the matrix instruction's sums (whose error against
-// the exact sum is about 1e-6 |q||x|): a streaming scan for a few queries, bound by reading the rows once (for one query
-// the whole search is its one launch), or the tile kernel with the candidate buffers of the 16-bit kernels (mfma_common.h).  The second sums those candidates' products in 64 bits -
-// every product of two codes is exact in fp32 and the scales are powers of two, so the sum is exact or off by a rounding of
-// 2^-53 - and sorts them by that, ties by the lower id.  A query therefore gets the same ids and scores in any batch.
+// The answer is the k best rows by the exact sums: score descending, ties by the lower id.  Three passes.  The first keeps, for every query, the
+// best k + 16 rows by the matrix cores' fp32 sums: a streaming scan for a few queries, bound by reading the rows once (for one query
+// its launch carries the second pass), or the tile kernel with the candidate buffers of the 16-bit kernels (mfma_common.h).  The second sums those
+// candidates' products in 64 bits - every product of two codes is exact in fp32 and the scales are powers of two, so the sum is exact or off by a
+// rounding of 2^-53 - and sorts them by that.  It also proves the list: a row that is not on it has a first-pass sum of at most the last one's, and
+// an exact one that is higher by the first pass's error at most, which goes by the row's length.  A row that is too short to make up for the gap
+// between the k-th exact score and the last sum is not among the k best.  The third pass takes the queries that some row is long enough for - more
+// than 16 rows within some 1e-5 |q||x| of the k-th score, copies of a row above all, or rows far longer than the others - and
+// sums those rows in 64 bits.  A query therefore gets the same ids and scores in any batch.
 //
 // Same place on the path as the 16-bit kernels: faiss.IndexFlatIP.search as called from core/index_manager.py:371.
 #include "f8_pp.h"
@@ -40,10 +44,54 @@ __device__ __forceinline__ double dot16(const i32x4_t& x, const i32x4_t& y) {
     }
     return (double)__fsub_rn(S, S0) + (double)L;
 }
-__device__ __forceinline__ void finish_query(const F8View& V, const unsigned char* qc, const unsigned char* qsc, const int64_t* ids, int kp, int k,
-                                             float* D, int64_t* I, int64_t id_offset, unsigned min_ord, double* score, int64_t* cid) {
+//
+// How far a sum of the first pass may be off for a query and a row of lengths q and x: f8_relative(blocks) q x + 2^-118 (q + x) + 2^-125, as long
+// as it cannot leave fp32.  An instruction adds 16 products per chain of roundings, eight of them to a block (f8_tile.h: 1.25 * 2^-23 of the
+// magnitudes at hand each, which are q x at most), and the scan joins two chains at the end.  The rest: values below 2^-133 and products below
+// the smallest fp32.  Solved for the length from which on a row may be off by `gap`:
+__device__ __forceinline__ double f8_relative(int blocks) { return (8 * blocks + 8) * (1.25 / 8388608.0); }
+__device__ __forceinline__ float f8_from(int blocks, double q, double gap) {
+    if (!(q < 1e37)) return 0.f;   // sums may leave fp32 whatever the row
+    const double x = (gap - 0x1p-118 * q - 0x1p-125) / (f8_relative(blocks) * q + 0x1p-118);
+    return x > 0.0 ? (float)(fmin(fmin(x, 1e37), 1e37 / fmax(q, 1e-300)) * (1 - 0x1p-20)) : 0.f;
+}
+// a score of the sorted list; the score floor cuts a suffix of it
+__device__ __forceinline__ void put_result(const F8ScanArgs& A, float* D, int64_t* I, int rank, double s, int64_t id) {
+    const float f = (float)s;
+    const bool keep = f32_to_ord(f) >= A.min_ord;
+    D[rank] = keep ? f : SSMI_NEG_MAX;
+    I[rank] = keep ? id + A.id_offset : -1;
+}
+// the LDS words that a query's second pass needs besides its sort: kp scores, kp ids of its own and kp that it is given, then these
+struct F8Proof { double qq, kth; skey_t last; };   // |q|^2, the k-th exact score, the last key of a full list (else 0)
+__host__ __device__ inline size_t finish_bytes(int kp) { return (size_t)kp * 24 + sizeof(F8Proof); }
+struct F8Scratch {
+    double* score;
+    int64_t *cid, *ids;
+    F8Proof* proof;
+    __device__ __forceinline__ F8Scratch(void* lds, int kp) : score(static_cast<double*>(lds)), cid(reinterpret_cast<int64_t*>(score + kp)), ids(cid + kp), proof(reinterpret_cast<F8Proof*>(ids + kp)) {}
+};
+__device__ __forceinline__ void finish_query(const F8ScanArgs& A, long long qi, const unsigned char* qc, const unsigned char* qsc, const F8Scratch& L) {
     constexpr int N = 4;
+    const F8View& V = A.v;
+    const int kp = A.kp, k = A.k;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), nwaves = blockDim.x >> 6;
+    double* score = L.score;
+    int64_t* cid = L.cid;
+    const int64_t* ids = L.ids;
+    float* D = A.D + qi * k;
+    int64_t* I = A.I + qi * k;
+    if (wave == nwaves - 1) {
+        double qq = 0.0;
+        for (int e = lane * 16; e < V.X.ld; e += 1024) {
+            const i32x4_t y = *reinterpret_cast<const i32x4_t*>(qc + e);
+            const double sq = (double)f8_scale(qsc[e / kF8Block]);
+            qq += dot16(y, y) * (sq * sq);
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) qq += __shfl_xor(qq, d);
+        if (lane == 0) L.proof->qq = qq;
+    }
     const long long seg_mask = (1ll << V.X.seg_shift) - 1;
     for (int c0 = wave * N; c0 < kp; c0 += nwaves * N) {
         const unsigned char* xc[N];
@@ -99,20 +147,28 @@ __device__ __forceinline__ void finish_query(const F8View& V, const unsigned cha
             rank += __builtin_popcountll(__builtin_amdgcn_ballot_w64(o < kp && io >= 0 && (so > s || (so == s && io < id))));
         }
         if (lane == 0 && rank < k) {
-            const float f = (float)s;
-            const bool keep = f32_to_ord(f) >= min_ord;   // the score floor cuts a suffix of the sorted list
-            D[rank] = keep ? f : SSMI_NEG_MAX;
-            I[rank] = keep ? id + id_offset : -1;
+            put_result(A, D, I, rank, s, id);
+            if (rank == k - 1) L.proof->kth = s;
         }
     }
     for (int c = valid + threadIdx.x; c < k; c += blockDim.x) { D[c] = SSMI_NEG_MAX; I[c] = -1; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const F8Proof& p = *L.proof;
+        // The list may lack a row whose sum came out at its last one's or below (a list that is not full: only one that left fp32).  Such a row is
+        // among the k best only if it gained the gap.  (A query that is NaN has no results.)
+        const double gap = p.last == 0 ? __builtin_inf() : valid >= k ? p.kth - (double)key_score(p.last) : -__builtin_inf();
+        const float from = f8_from(V.X.ld / kF8Block, sqrt(p.qq) * (1 + 0x1p-40), gap);
+        const bool proven = p.qq != p.qq || *A.longest < from;
+        A.state[qi] = F8State{valid >= k ? p.kth : -__builtin_inf(), from, proven ? 0u : 1u, 0u, 0u};
+    }
 }
 
 // ---- between the passes: the first pass's lists of one query -> its kp best rows.  All threads of the workgroup ----
 // The lists' m-th keys, m = ceil(kp / P), bound the kp-th best from below: if c = ceil(kp / m) of them reach a score, m c >= kp
 // rows do.  (For kp <= 48 the lane maxima of the heads serve, 64 values instead of P.)  The keys at or above the bound, two or
 // three times kp of the P kp, are collected and sorted.  A full merge of 256 lists of 216 keys took 100 us on one workgroup.
-// keys: LDS, nwaves * 64 R words and at least kSurvivors + 2; ids: kp words of LDS.
+// keys: LDS, nwaves * 64 R words and at least kSurvivors + 2.
 static constexpr int kSurvivors = 2048;
 template <int RV>
 __device__ __forceinline__ unsigned nth_score(const skey_t* lists, int P, int kp, int m, int c) {
@@ -127,7 +183,7 @@ __device__ __forceinline__ unsigned nth_score(const skey_t* lists, int P, int kp
     return t.kth(c);
 }
 template <int R>
-__device__ __forceinline__ void merge_to_ids(const skey_t* lists, int P, int kp, skey_t* keys, int64_t* ids) {
+__device__ __forceinline__ void merge_to_ids(const skey_t* lists, int P, int kp, skey_t* keys, const F8Scratch& L) {
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), nwaves = blockDim.x >> 6;
     unsigned* word = reinterpret_cast<unsigned*>(keys);   // [0] bound, [1] survivors
     skey_t* surv = keys + 1;
@@ -196,7 +252,8 @@ __device__ __forceinline__ void merge_to_ids(const skey_t* lists, int P, int kp,
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int e = r * 64 + lane;
-            if (e < kp) ids[e] = t.v[r] ? (int64_t)key_id(t.v[r]) : -1;
+            if (e < kp) L.ids[e] = t.v[r] ? (int64_t)key_id(t.v[r]) : -1;
+            if (e == kp - 1) L.proof->last = t.v[r];
         }
     }
     __syncthreads();
@@ -243,20 +300,210 @@ __global__ void __launch_bounds__(1024) f8_finish_kernel(F8ScanArgs A, int P) {
     unsigned char* qs = smem;
     unsigned char* qsc = smem + ld;
     skey_t* keys = reinterpret_cast<skey_t*>(smem + (ld + ld / kF8Block + 15) / 16 * 16);
-    double* score = reinterpret_cast<double*>(reinterpret_cast<unsigned char*>(keys) + merge_keys_bytes(blockDim.x >> 6, R));
-    int64_t* cid = reinterpret_cast<int64_t*>(score + kp);
-    int64_t* ids = cid + kp;
+    const F8Scratch L(reinterpret_cast<unsigned char*>(keys) + merge_keys_bytes(blockDim.x >> 6, R), kp);
     if (A.shared && threadIdx.x == 0) A.shared[qi] = 0;   // as the next launch expects it
     stage_query(A, qi, qs, qsc);
-    merge_to_ids<R>(A.partial + (size_t)qi * P * kp, P, kp, keys, ids);
-    finish_query(A.v, qs, qsc, ids, kp, A.k, A.D + qi * A.k, A.I + qi * A.k, A.id_offset, A.min_ord, score, cid);
+    merge_to_ids<R>(A.partial + (size_t)qi * P * kp, P, kp, keys, L);
+    finish_query(A, qi, qs, qsc, L);
+}
+
+// ---- third pass: the queries that are not proven, over all rows.  A workgroup per CU ----
+// Scores as finish_query's.  W workgroups share a query (all of the grid if it is alone), each takes a range of the rows, picks those that are
+// long enough and keeps what may be among the k best in LDS, sorted down to k whenever the buffer fills; the last to finish joins their lists.  1M x 4096 with every row long enough: 1.4 ms
+// for one query, 0.8 ms for each of many, by the vector units (four instructions a product).  With nothing to do the launch costs 3 us.
+static constexpr int kExactThreads = 1024, kExactEntries = 2048, kExactRound = 256;   // entries of a buffer, and how many a round may add
+struct F8Exact {
+    double* score;
+    unsigned *id, *count;   // count[0] entries, count[1] a flag
+    double thr;             // entries have to beat (thr, thr_id)
+    unsigned thr_id;
+    __device__ __forceinline__ bool beats(double s, unsigned i) const { return s > thr || (s == thr && i < thr_id); }
+    __device__ __forceinline__ void add(double s, unsigned i) const {
+        const unsigned pos = atomicAdd(count, 1u);
+        score[pos] = s;
+        id[pos] = i;
+    }
+    // down to the k best, in order.  All threads; their entries are there
+    __device__ __forceinline__ int shrink(int k) {
+        const int n = (int)*count;
+        int all = 64;
+        while (all < n) all <<= 1;
+        for (int e = n + threadIdx.x; e < all; e += blockDim.x) { score[e] = -__builtin_inf(); id[e] = 0xffffffffu; }
+        for (int size = 2; size <= all; size <<= 1)
+            for (int gap = size >> 1; gap; gap >>= 1) {
+                __syncthreads();
+                for (int t = threadIdx.x; t < all / 2; t += blockDim.x) {
+                    const int a = (t / gap) * 2 * gap + t % gap, b = a + gap;
+                    const double sa = score[a], sb = score[b];
+                    const unsigned ia = id[a], ib = id[b];
+                    const bool first = sa > sb || (sa == sb && ia < ib);
+                    if (first != ((a & size) == 0)) {
+                        score[a] = sb; score[b] = sa;
+                        id[a] = ib; id[b] = ia;
+                    }
+                }
+            }
+        __syncthreads();
+        const int left = min(n, k);
+        if (n >= k) { thr = score[k - 1]; thr_id = id[k - 1]; }
+        if (threadIdx.x == 0) *count = (unsigned)left;
+        __syncthreads();
+        return left;
+    }
+    // a round's entries are in: make room for the next
+    __device__ __forceinline__ void next_round(int k) {
+        __syncthreads();
+        const bool fill = *count > (unsigned)(kExactEntries - kExactRound);
+        __syncthreads();   // everybody has looked before anybody adds
+        if (fill) shrink(k);
+    }
+};
+__global__ void __launch_bounds__(kExactThreads) f8_exact_kernel(F8ScanArgs A) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    const F8View& V = A.v;
+    const int ld = V.X.ld, k = A.k, nq = (int)A.q.n;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), nwaves = blockDim.x >> 6;
+    F8Exact X;
+    X.score = reinterpret_cast<double*>(smem);
+    X.id = reinterpret_cast<unsigned*>(X.score + kExactEntries);
+    X.count = X.id + kExactEntries;
+    unsigned short* open = reinterpret_cast<unsigned short*>(X.count + 4);   // [kF8Batch] the queries that are left
+    unsigned* sel = reinterpret_cast<unsigned*>(open + kF8Batch);            // [blockDim.x] rows of a round
+    unsigned char* qs = reinterpret_cast<unsigned char*>(sel + blockDim.x);
+    unsigned char* qsc = qs + ld;
+    if (wave == 0) {
+        int n = 0;
+        for (int q0 = 0; q0 < nq; q0 += 64) {
+            const bool is = q0 + lane < nq && __hip_atomic_load(&A.state[q0 + lane].ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
+            const unsigned long long m = __builtin_amdgcn_ballot_w64(is);
+            if (is) open[n + __builtin_popcountll(m & ((1ull << lane) - 1))] = (unsigned short)(q0 + lane);
+            n += __builtin_popcountll(m);
+        }
+        if (lane == 0) X.count[1] = (unsigned)n;
+    }
+    __syncthreads();
+    const int nopen = (int)X.count[1];
+    if (nopen == 0) return;
+    const int W = max(1, (int)gridDim.x / nopen);
+    // lanes that share a row: 16 codes each, added up in finish_query's order, so that a row has one score
+    const int lpr = ld > 512 ? 64 : ld > 256 ? 32 : ld > 128 ? 16 : 8, rpw = 64 / lpr, sub = lane / lpr, off = (lane % lpr) * 16;
+    const long long seg_mask = (1ll << V.X.seg_shift) - 1;
+    for (int item = blockIdx.x; item < nopen * W; item += gridDim.x) {
+        const int u = item / W, part = item % W;
+        const long long qi = open[u];
+        float* D = A.D + qi * k;
+        int64_t* I = A.I + qi * k;
+        __syncthreads();   // the query before is done with
+        if (threadIdx.x == 0) X.count[0] = X.count[1] = 0;
+        stage_query(A, qi, qs, qsc);
+        X.thr = A.state[qi].edge;
+        X.thr_id = 0xffffffffu;
+        __syncthreads();
+        const float from = A.state[qi].from;
+        const long long begin = V.X.nrows * part / W, end = V.X.nrows * (part + 1) / W;
+        for (long long r0 = part == 0 ? begin - (long long)blockDim.x : begin; r0 < end; r0 += blockDim.x) {
+            // the rows that are long enough (a NaN's -1 is not), and before them the second pass's results that are not
+            const bool listed = r0 < begin;
+            const int e = threadIdx.x;
+            if (listed ? e < k && !(I[e] == -1 && D[e] == SSMI_NEG_MAX) : r0 + e < end) {
+                const long long row = listed ? I[e] - A.id_offset : r0 + e;
+                const float len = static_cast<const float*>(V.lsegs[row >> V.X.seg_shift])[row & seg_mask];
+                if ((len >= from) != listed) sel[atomicAdd(X.count + 1, 1u)] = (unsigned)row;
+            }
+            __syncthreads();
+            const int nsel = (int)X.count[1];
+            for (int s0 = 0; s0 < nsel; s0 += kExactRound) {
+                for (int t = s0 + wave * rpw; t < min(nsel, s0 + kExactRound); t += nwaves * rpw) {
+                    const unsigned row = sel[min(t + sub, nsel - 1)];
+                    const long long seg = row >> V.X.seg_shift, in = row & seg_mask;
+                    const unsigned char* xc = static_cast<const unsigned char*>(V.X.segs[seg]) + in * ld;
+                    const unsigned char* xs = static_cast<const unsigned char*>(V.ssegs[seg]) + in * V.sld;
+                    double sum = 0.0;
+#pragma unroll 4
+                    for (int e = off; e < ld; e += lpr * 16) {
+                        const int blk = e / kF8Block;
+                        sum += dot16(*reinterpret_cast<const i32x4_t*>(xc + e), *reinterpret_cast<const i32x4_t*>(qs + e)) * ((double)f8_scale(qsc[blk]) * (double)f8_scale(xs[blk]));
+                    }
+                    for (int d = lpr >> 1; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
+                    if (off == 0 && t + sub < nsel && X.beats(sum, row)) X.add(sum, row);
+                }
+                X.next_round(k);
+            }
+            if (threadIdx.x == 0) X.count[1] = 0;
+            __syncthreads();
+        }
+        int n = X.shrink(k);
+        if (W > 1) {
+            // (A.lists: W k entries for each of the queries, filled by whoever is done)
+            F8Entry* list = A.lists + (size_t)u * W * k;
+            F8State* st = A.state + qi;
+            if (threadIdx.x == 0) X.count[1] = __hip_atomic_fetch_add(&st->pos, (unsigned)n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            const unsigned pos = X.count[1];
+            for (int e = threadIdx.x; e < n; e += blockDim.x) list[pos + e] = F8Entry{X.score[e], (long long)X.id[e]};
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) X.count[1] = __hip_atomic_fetch_add(&st->ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (X.count[1] != (unsigned)W) return;   // (a grid with W > 1 has one item a workgroup)
+            __threadfence();
+            const int total = (int)__hip_atomic_load(&st->pos, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (threadIdx.x == 0) X.count[0] = 0;
+            X.thr = -__builtin_inf();
+            X.thr_id = 0xffffffffu;
+            __syncthreads();
+            for (int e0 = 0; e0 < total; e0 += kExactRound) {
+                const int e = e0 + threadIdx.x;
+                if (threadIdx.x < kExactRound && e < total) {
+                    const F8Entry v = list[e];
+                    if (X.beats(v.score, (unsigned)v.id)) X.add(v.score, (unsigned)v.id);
+                }
+                X.next_round(k);
+            }
+            n = X.shrink(k);
+        }
+        for (int e = threadIdx.x; e < k; e += blockDim.x) {
+            if (e < n) put_result(A, D, I, e, X.score[e], (int64_t)X.id[e]);
+            else { D[e] = SSMI_NEG_MAX; I[e] = -1; }
+        }
+    }
+}
+
+// lengths of rows: the waves take groups of rows as above
+__global__ void __launch_bounds__(256) f8_lengths_kernel(F8Mat m, int ld, float* lengths, unsigned* longest) {
+    const int lane = lane_id(), wave = threadIdx.x >> 6;
+    const int lpr = ld > 512 ? 64 : ld > 256 ? 32 : ld > 128 ? 16 : 8, rpw = 64 / lpr, sub = lane / lpr, off = (lane % lpr) * 16;
+    float most = 0.f;
+    for (long long r0 = ((long long)blockIdx.x * 4 + wave) * rpw; r0 < m.n; r0 += (long long)gridDim.x * 4 * rpw) {
+        const long long row = min(r0 + sub, m.n - 1);
+        double sum = 0.0;
+#pragma unroll 2
+        for (int e = off; e < ld; e += lpr * 16) {
+            const i32x4_t x = *reinterpret_cast<const i32x4_t*>(m.codes + row * m.stride + e);
+            const double s = (double)f8_scale(m.scales[row * m.sstride + e / kF8Block]);
+            sum += dot16(x, x) * (s * s);
+        }
+        for (int d = lpr >> 1; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
+        const float len = sum >= 0.0 ? (float)(sqrt(sum) * (1 + 0x1p-22)) : -1.f;   // (beyond fp32: infinite)
+        if (off == 0 && r0 + sub < m.n) lengths[row] = len;
+        most = fmaxf(most, len);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    if (lane == 0 && most > 0.f) atomicMax(longest, __float_as_uint(most));
+}
+hipError_t launch_f8_lengths(const F8Mat& m, int ld, float* lengths, unsigned* longest, int num_cu, hipStream_t s) {
+    if (m.n <= 0) return hipSuccess;
+    const long long blocks = (m.n + 3) / 4, most = (long long)num_cu * 8;
+    hipLaunchKernelGGL(f8_lengths_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, m, ld, lengths, longest);
+    return hipGetLastError();
 }
 
 // ---- streaming scan: up to BT <= 8 queries ----
 // Bound by reading the rows once; what reads fastest decides the layout.  A plain read of 1M x 4096 codes ran at 5.9 TB/s with
 // 16 rows x 64 bytes per load instruction (the operand layout of the 16x16x128 instruction as it is) and at 6.7-7.0 TB/s with 8
 // rows x 128 bytes, non-temporal loads and 4-8 waves per CU.  So one load is one whole block of eight rows, 16 codes a lane,
-// and feeds the low half of one instruction whose high half is zero (the matrix pipe is 7 % busy): the sixteen operand rows
+// and feeds two instructions of K = 32 (f8_tile.h): the sixteen operand rows
 // are the 8 rows x {even, odd 16-byte chunks}, the sixteen columns 8 queries x {even, odd chunks}, and a score is the
 // sum of the even-even and the odd-odd element of the result.  Columns beyond BT repeat a query and are never looked at.
 // Up to eight loads (8 KiB) per stage and wave, three stages in flight: NB = 0: a stage is up to eight blocks of one group of
@@ -491,11 +738,9 @@ __global__ void __launch_bounds__(512) f8_scan_kernel(F8ScanArgs A) {
     if (!tail_last_block(A.counter, gridDim.x, reinterpret_cast<unsigned*>(keys))) return;
     // one query: the last workgroup goes on (several queries have a workgroup each: f8_finish_kernel)
     if (threadIdx.x == 0) A.shared[0] = 0;   // as the next launch expects it
-    double* score = reinterpret_cast<double*>(reinterpret_cast<unsigned char*>(keys) + merge_keys_bytes(nwaves, R));
-    int64_t* cid = reinterpret_cast<int64_t*>(score + kp);
-    int64_t* ids = cid + kp;
-    merge_to_ids<R>(A.partial, (int)gridDim.x, kp, keys, ids);
-    finish_query(V, qs, qsc, ids, kp, A.k, A.D, A.I, A.id_offset, A.min_ord, score, cid);
+    const F8Scratch L(reinterpret_cast<unsigned char*>(keys) + merge_keys_bytes(nwaves, R), kp);
+    merge_to_ids<R>(A.partial, (int)gridDim.x, kp, keys, L);
+    finish_query(A, 0, qs, qsc, L);
 }
 
 // the k-th score of any slice bounds the final one: the slices share the highest (mfma.hip).  A wave's own queries, as in the folds
@@ -529,8 +774,8 @@ __device__ __forceinline__ void seed_thresholds(const float* maxima, int wave, i
 }
 
 // ---- tile kernel: 256 rows x TQ queries per workgroup, a slice of the rows each ----
-// Bound by the rows' way from memory while the batch is small (1M x 4096: 16 queries 865 us, 4.8 TB/s; 64 queries 988 us, 4.2), by the
-// folds and the first tile of a slice over few rows (10000 x 4096, 64 queries: 71 us, of which this kernel 52).
+// Bound by the rows' way from memory while the batch is small (1M x 4096: 16 queries 791 us, 5.2 TB/s; 64 queries 933 us, 4.4), by the
+// folds and the first tile of a slice over few rows (10000 x 4096, 64 queries: 87 us).
 template <int MT, int NT, int WM, int WN, int R>
 __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, MfmaParams P) {
     using T = F8Tile<MT, NT, WM, WN, 3>;
@@ -654,7 +899,7 @@ __device__ __forceinline__ void filter_big(const F8Pp::Acc& acc, int row_base, i
 
 // A workgroup keeps its query tile and walks a slice of the rows; the first slab of the next row tile travels under this one's filter.
 // Folds, thresholds and the bound from the slices' published tops are those of the 16-bit kernel (mfma_pp.hip).
-// 1M x 4096, 1024 queries: 3.93 ms, 2.13 PFLOP/s (2.41 for the product alone, f8_matmul.hip); 256 queries: 1.37 ms - one slab ahead of the
+// 1M x 4096, 1024 queries: 6.65 ms, 1.26 PFLOP/s (1.55 for the product alone, f8_matmul.hip); 256 queries: 1.93 ms - one slab ahead of the
 // products does not cover the way from memory where no second query tile shares the rows.
 template <int R>
 __global__ void __launch_bounds__(512, 2) f8_search_big_kernel(F8View V, F8Mat q, MfmaParams P) {
@@ -779,15 +1024,16 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
         const auto rows = [&](int turns) { return (3 * turns + stages - 1) / stages * run_rows * waves; };
         p->cap = std::max(4096 / p->bt, rows(1) + 64);
         for (p->every = 1; rows(2 * p->every) + 64 <= p->cap;) p->every *= 2;
-        const size_t work = std::max((size_t)p->bt * p->cap * sizeof(skey_t), p->bt > 1 ? 0 : merge_keys_bytes(waves, p->r) + (size_t)p->kp * 24);
+        const size_t work = std::max((size_t)p->bt * p->cap * sizeof(skey_t), p->bt > 1 ? 0 : merge_keys_bytes(waves, p->r) + finish_bytes(p->kp));
         p->lds = (p->bt * per_query + 15) / 16 * 16 + 64 + (size_t)p->bt * 64 * p->r * sizeof(skey_t) + work;
         p->grid_x = (int)std::min<long long>(num_cu, (runs + waves - 1) / waves);
         p->parts = p->grid_x;
         p->kernel = "f8_scan_kernel";
     } else {
         // Over few rows narrow tiles of queries win: more workgroups, fewer lists each.  Up to seven rounds of the chip (us in tiles of 64, 128 and
-        // 256 queries: 10000 x 4096, 256 queries 74, 102, 169; 20000 x 4096, 512 queries 147, 175, 180; 100000 x 4096, 256 queries 299, 312, 371, 512
-        // queries 471, 422, 472, 1024 queries 797, 678, 630; 1M x 4096, 256 queries 1809, 1540, 1349)
+        // 256 queries: 10000 x 4096, 256 queries 89, 127, 205; 20000 x 4096, 512 queries 199, 221, 217; 50000 x 4096, 256 queries 232, 220, 346, 1024
+        // queries 611, 581, 589; 100000 x 4096, 256 queries 362, 368, 377, 512 queries 602, 556, 583, 1024 queries 1082, 951, 887; 100000 x 768,
+        // 256 queries 178, 203, 291; 1M x 4096, 256 queries 2547, 2245, 1965)
         const long long tiles = (nrows + 255) / 256;
         const auto few = [&](int tq) { return tiles * ((nq + tq - 1) / tq) <= 7ll * num_cu; };
         p->tq = nq <= 64 || few(64) ? 64 : nq <= 128 || few(128) ? 128 : 256;
@@ -832,7 +1078,7 @@ template <int R>
 static hipError_t launch_finish_r(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s) {
     const int threads = R == 16 ? 256 : 512;   // (the lists of the waves meet in LDS)
     const int ld = a.v.X.ld;
-    const size_t lds = (size_t)(ld + ld / kF8Block + 15) / 16 * 16 + merge_keys_bytes(threads / 64, R) + (size_t)p.kp * 24;
+    const size_t lds = (size_t)(ld + ld / kF8Block + 15) / 16 * 16 + merge_keys_bytes(threads / 64, R) + finish_bytes(p.kp);
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_finish_kernel<R>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
@@ -849,6 +1095,16 @@ hipError_t launch_f8_finish(const F8ScanArgs& a, const F8SearchPlan& p, hipStrea
         case 16: return launch_finish_r<16>(a, p, s);
     }
     return hipErrorInvalidValue;
+}
+hipError_t launch_f8_exact(const F8ScanArgs& a, int num_cu, hipStream_t s) {
+    const int ld = a.v.X.ld;
+    const size_t lds = kExactEntries * 12 + 16 + kF8Batch * 2 + kExactThreads * 4 + (size_t)(ld + ld / kF8Block + 15) / 16 * 16;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_exact_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(f8_exact_kernel, dim3((unsigned)num_cu), dim3(kExactThreads), lds, s, a);
+    return hipGetLastError();
 }
 hipError_t launch_f8_scan(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s) {
     switch (p.r * 16 + p.bt) {

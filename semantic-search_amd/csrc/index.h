@@ -26,7 +26,7 @@ struct RowStore {
     void** d_segs = nullptr;
 
     int init(int d, int dtype, hipStream_t stream);  // `stream`: where the segment table is zeroed (see zero_device_sync)
-    int init_scales(const RowStore& codes, hipStream_t stream);  // 8-bit rows: the scale bytes of `codes`, segment by segment
+    int init_side(const RowStore& codes, int bytes, hipStream_t stream);  // 8-bit rows: `bytes` beside every row of `codes`, segment by segment
     void destroy();
     int reserve(long long total_rows, hipStream_t stream);
     RowView view() const;
@@ -40,6 +40,8 @@ struct ssmi_index {
     int num_cu = 256;
     ssmi::RowStore rows;  // Flat: the database.  IVF: the slot store (pages of list members)
     ssmi::RowStore scales;  // SSMI_F8: one scale byte per 128 codes of `rows` (f8.h); rows and segments as there
+    ssmi::RowStore lengths;  // SSMI_F8: the length of every row, an fp32 rounded up (f8_search.hip proves its lists with them)
+    float* f8_longest = nullptr;  // ... and the largest of them (device)
     // fp16 copy of an fp32 Flat database, built lazily by the first large-batch search so that
     // it can run on the MFMA kernel (costs +50 % HBM; batch-1..8 searches keep using the fp32 rows)
     ssmi::RowStore shadow16;

@@ -55,3 +55,123 @@ def test_products_that_cancel_leave_the_others(ssa, m, n, k):
     want = (x.double() @ y.double().T).bfloat16()
     assert torch.equal(ssa.matmul_f8(a, b), want)
     assert (want > 0).all()
+
+
+def exact_search(rows, queries, k):
+    """Score descending, ties by the lower id, over the 64-bit products of what the 8-bit rows stand for (none is NaN)."""
+    S = queries.dequantize().double() @ rows.dequantize().double().T
+    best, ids = torch.sort(S, dim=1, descending=True, stable=True)
+    return best[:, :k], ids[:, :k]
+
+
+def check_search(ssa, rows, queries, k):
+    index = ssa.IndexFlatIP(rows.d, storage="f8")
+    index.add(rows)
+    D, I = index.search(queries, k)
+    best, ids = exact_search(rows, queries, k)
+    kk = best.shape[1]
+    A, B = queries.dequantize().double(), rows.dequantize().double()
+    # a 64-bit sum in another order may part in its last bits: rows may trade places there and nowhere else
+    slack = 1e-13 * (A.norm(dim=1, keepdim=True) * B.norm(dim=1).max())
+    got = (A @ B.T).gather(1, I[:, :kk])
+    assert ((got - best).abs() <= slack).all()
+    assert ((I[:, :kk] == ids) | ((got - best).abs() <= slack)).all()
+    assert ((D[:, :kk].double() - best).abs() <= best.abs() * 2.0 ** -24 + slack).all()
+    assert (I[:, kk:] == -1).all()
+    assert all(len(set(r)) == kk for r in I[:, :kk].tolist())
+    index.close()
+    return I
+
+
+@pytest.mark.parametrize("n,d", [(20000, 512), (6000, 768), (3000, 1024), (30000, 128)])
+@pytest.mark.parametrize("channels,share", [(1, 0.5), (1, 0.98), (3, 0.98), (8, 0.98), (4, 0.9999)])
+@pytest.mark.parametrize("nq,k", [(1, 1), (1, 10), (1, 100), (1, 1008), (8, 1), (8, 10), (20, 1), (20, 10), (20, 100), (128, 1), (128, 10), (128, 100),
+                                  (300, 1), (300, 10), (300, 100), (300, 1008)])
+def test_search_of_rows_with_strong_channels(ssa, n, d, channels, share, nq, k):
+    """Unit rows, `share` of whose length lies in a few channels, as raw last hidden states have it."""
+    g = torch.Generator(device="cuda").manual_seed(SALT + n + d + channels)
+    make = lambda c: torch.nn.functional.normalize(torch.randn(c, d, generator=g, device="cuda"))  # noqa: E731
+    x, q = make(n), make(nq)
+    where = list(range(5, 5 + 8 * channels, 8)) if channels < 8 else list(range(8, 8 + channels))   # apart, or side by side
+    for v in (x, q):
+        v *= (1 - share * share) ** 0.5
+        v[:, where] = share / channels ** 0.5 * (1 + 0.01 * torch.randn(len(v), channels, generator=g, device="cuda"))
+    check_search(ssa, ssa.quantize_f8(x), ssa.quantize_f8(q), k)
+
+
+@pytest.mark.parametrize("nq", [1, 3, 8, 20, 100, 300])
+@pytest.mark.parametrize("n,d,k", [(5000, 300, 10), (3000, 4096, 100), (70000, 128, 30), (40, 200, 10)])
+def test_search_among_rows_that_hardly_differ(ssa, n, d, k, nq):
+    """More rows than there are spare candidates within a rounding of fp32 of each other: their order is that of the exact sums."""
+    g = torch.Generator(device="cuda").manual_seed(SALT + n + d)
+    x = torch.randn(1, d, generator=g, device="cuda").repeat(n, 1)
+    q = torch.randn(nq, d, generator=g, device="cuda")
+    few = torch.arange(0, d, 7, device="cuda")
+    x[:, 0], q[:, 0] = 400.0, 400.0
+    x[:, few[1:]] = torch.randint(-3, 4, (n, len(few) - 1), generator=g, device="cuda").float() * 2.0 ** -6   # they differ here,
+    q[:, few[1:]] = torch.randint(-3, 4, (nq, len(few) - 1), generator=g, device="cuda").float() * 2.0 ** -6  # and by 2^-12 in 160000
+    check_search(ssa, ssa.quantize_f8(x), ssa.quantize_f8(q), k)
+
+
+@pytest.mark.parametrize("nq", [1, 5, 40, 300])
+@pytest.mark.parametrize("n,k", [(9000, 1), (9000, 20), (9000, 1008), (300, 300)])
+def test_search_among_copies_returns_the_lowest_ids(ssa, n, k, nq):
+    """The whole index is copies of five rows: ties that no list of candidates holds."""
+    g = torch.Generator(device="cuda").manual_seed(SALT + n + k)
+    few = torch.nn.functional.normalize(torch.randn(5, 260, generator=g, device="cuda"))
+    which = torch.randint(0, 5, (n,), generator=g, device="cuda")
+    x, q = ssa.quantize_f8(few[which]), ssa.quantize_f8(torch.randn(nq, 260, generator=g, device="cuda"))
+    I = check_search(ssa, x, q, k)
+    S = q.dequantize().double() @ ssa.quantize_f8(few).dequantize().double().T
+    order = S.argsort(dim=1, descending=True)
+    for i in range(min(nq, 10)):
+        want = torch.cat([(which == c).nonzero()[:, 0] for c in order[i]])[:k]
+        assert torch.equal(I[i], want)
+
+
+@pytest.mark.parametrize("scale_x,scale_q", [(1e37, 1.0), (1e30, 1e30), (1e-37, 1.0), (1e-20, 1e-20), (3e38, 1e-38)])
+@pytest.mark.parametrize("nq", [1, 20, 300])
+def test_search_at_the_ends_of_fp32(ssa, scale_x, scale_q, nq):
+    """Sums that leave fp32 on the way, or vanish in it: the answer is the 64-bit one (what fp32 cannot hold of it: infinite or 0)."""
+    g = torch.Generator(device="cuda").manual_seed(SALT + nq)
+    x, q = (torch.nn.functional.normalize(torch.randn(c, 200, generator=g, device="cuda")) for c in (2000, nq))
+    rows, queries = ssa.quantize_f8(x * scale_x), ssa.quantize_f8(q * scale_q)
+    index = ssa.IndexFlatIP(200, storage="f8")
+    index.add(rows)
+    D, I = index.search(queries, 10)
+    A = torch.from_numpy(plain.values(queries.codes.view(torch.uint8).cpu().numpy(), queries.scales.cpu().numpy(), 200))
+    B = torch.from_numpy(plain.values(rows.codes.view(torch.uint8).cpu().numpy(), rows.scales.cpu().numpy(), 200))
+    best, ids = torch.sort(A @ B.T, dim=1, descending=True, stable=True)
+    assert torch.equal(I.cpu(), ids[:, :10])
+    want = best[:, :10].float()
+    assert ((D.cpu() == want) | ((D.cpu() - want).abs() <= want.abs() * 2.0 ** -22 + 2.0 ** -149)).all()
+
+
+@pytest.mark.parametrize("nq", [1, 8, 40, 300])
+@pytest.mark.parametrize("where", [[777], [0, 2999], list(range(100, 400))])
+def test_search_among_rows_of_very_different_lengths(ssa, where, nq):
+    """Some rows a million times the others: what fp32 loses beside them is more than the gaps between the others' scores."""
+    g = torch.Generator(device="cuda").manual_seed(SALT)
+    x, q = (torch.nn.functional.normalize(torch.randn(c, 200, generator=g, device="cuda")) for c in (3000, nq))
+    x[where] *= 1e6
+    for k in (10, 200):
+        check_search(ssa, ssa.quantize_f8(x), ssa.quantize_f8(q), k)
+
+
+@pytest.mark.parametrize("offset", [-700, -1, 5, 1 << 40])
+@pytest.mark.parametrize("nq", [1, 30])
+def test_offsets_and_floors_of_queries_that_take_the_exact_pass(ssa, nq, offset):
+    g = torch.Generator(device="cuda").manual_seed(SALT + 3)
+    x, q = (torch.nn.functional.normalize(torch.randn(c, 200, generator=g, device="cuda")) for c in (3000, nq))
+    x[700:760] = x[700]          # copies for some,
+    x[5] *= 1e5                  # and a long row for all
+    rows, queries = ssa.quantize_f8(x), ssa.quantize_f8(q)
+    index = ssa.IndexFlatIP(200, storage="f8")
+    index.add(rows)
+    best, ids = exact_search(rows, queries, 100)
+    D, I = index.search(queries, 100, id_offset=offset)
+    assert torch.equal(I, ids + offset)
+    floor = float(best[0, 50])
+    Df, If = index.search(queries, 100, id_offset=offset, min_score=floor)
+    keep = D >= np.float32(floor)
+    assert torch.equal(If, torch.where(keep, I, -1)) and torch.equal(Df, torch.where(keep, D, torch.full_like(D, -np.finfo(np.float32).max)))
