@@ -211,7 +211,7 @@ int ssmi_f8_quantize(int device, int64_t n, int d, const void* x, int src_dtype,
 int ssmi_f8_dequantize(int device, int64_t n, int d, const uint8_t* codes, int64_t codes_stride, const uint8_t* scales,
                        int64_t scales_stride, void* out, int out_dtype, int64_t out_stride, void* stream);
 /* The norm that ends in 8-bit rows.  h = x + residual, rounded to dtype and stored in residual_out (which may be residual or x
- * itself); without a residual (NULL) h = x.  y = h / sqrt(mean(h^2) + eps) * weight (NULL: 1), in 64 bits and rounded to fp32; unit != 0:
+ * itself); without a residual (NULL) h = x.  y = h / sqrt(mean(h^2) + eps) * weight (NULL: 1), in 64 bits and rounded once, to its code; unit != 0:
  * y / max(|y|_2, 1e-12), what goes into an inner-product index.  codes / scales receive y.  d <= 16384. */
 int ssmi_f8_rms_norm(int device, int64_t n, int d, const void* x, int dtype, int64_t x_stride, const void* residual,
                      int64_t residual_stride, void* residual_out, int64_t residual_out_stride, const void* weight,

@@ -69,13 +69,23 @@ __device__ __forceinline__ void row_sums(double& a, double& b, double2* lds) {
     }
 }
 
+// 64 bits -> an fp32 whose last bit says that something was cut: rounding that again, to the four bits of a code, gives what rounding the
+// 64 bits gives, and a value above 448 s stays above it.  (To nearest twice: a code in about a million was one step off, or its block twice as
+// coarse.)  Below 2^-126 to nearest.
+__device__ __forceinline__ float narrow_odd(double y) {
+    unsigned long long b = (unsigned long long)__double_as_longlong(y);
+    unsigned lo = (unsigned)b;
+    lo = (lo | ((lo & 0x1fffffffu) + 0x1fffffffu)) & 0xe0000000u;   // (the addition carries into bit 29 unless all below are zero)
+    return (float)__longlong_as_double((long long)((b & 0xffffffff00000000ull) | lo));
+}
+
 // Eight elements per thread and pass: 16 threads hold a block of 128, so its maximum is four DPP steps and the codes leave as
 // 8 bytes per lane.  WAVE: a row per wave (rows up to 2048 elements, many of them), else a row per block.
-// The norm's sums and its one factor per row are 64-bit: y is then the exact value rounded once, and an element's code is that of
-// the exact row unless y lies within 2^-24 of a border.  (With fp32 sums and factors three times as many codes parted from the exact
-// ones; the 64-bit products hide behind memory.)  unit needs no second pass: |y| = f |h w| for y = f h w.
+// The norm's sums and its one factor per row are 64-bit and y is rounded once, to its code (narrow_odd): an element's code is that of the exact row
+// unless y lies within 2^-40 of a border.  (With fp32 sums and factors codes part from the exact ones a million times as often; the 64-bit products
+// hide behind memory.)  unit needs no second pass: |y| = f |h w| for y = f h w.
 // The quantiser is bound by memory (200000 x 2048 fp32: 376 us, 5.4 TB/s), the norm by what little of its rows is in flight while it
-// reduces (32768 x 4096 bf16 with a residual: 238 us, 4.0 TB/s; 200000 x 2048 fp32, unit: 445 us, 4.6 TB/s; a row of 4096 per wave
+// reduces (32768 x 4096 bf16 with a residual: 218 us, 4.3 TB/s; 200000 x 2048 fp32, unit: 479 us, 4.3 TB/s; a row of 4096 per wave
 // needs 254 registers and took 574 us).
 // (Four passes of 1024 threads would take rows of 32768 elements through the norm, but spill.)
 template <typename T, int ITER, bool WAVE, bool VEC, bool NORM>
@@ -141,7 +151,7 @@ __global__ void __launch_bounds__(WAVE ? 256 : 1024, WAVE ? 1 : 5) f8_rows_kerne
                     float w[8];
                     weights(c0 + (i * tpr + t) * 8, w);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[i][j] = (float)((double)v[i][j] * (double)w[j] * f);
+                    for (int j = 0; j < 8; ++j) v[i][j] = narrow_odd((double)v[i][j] * (double)w[j] * f);
                 }
             }
 #pragma unroll

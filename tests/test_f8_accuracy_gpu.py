@@ -175,3 +175,32 @@ def test_offsets_and_floors_of_queries_that_take_the_exact_pass(ssa, nq, offset)
     Df, If = index.search(queries, 100, id_offset=offset, min_score=floor)
     keep = D >= np.float32(floor)
     assert torch.equal(If, torch.where(keep, I, -1)) and torch.equal(Df, torch.where(keep, D, torch.full_like(D, -np.finfo(np.float32).max)))
+
+
+def norm_case(name, t):
+    g = torch.Generator(device="cuda").manual_seed(SALT + len(name))
+    n, d = {"odd rows": (1023, 777), "residual": (900, 4096), "long": (60, 16384), "dominant": (2000, 1000), "dominant long": (40, 15001), "narrow": (3000, 128)}[name]
+    x, r = (torch.randn(n, d, generator=g, device="cuda") for _ in range(2))
+    if "dominant" in name:
+        x[torch.arange(n), torch.randint(0, d, (n,), generator=g, device="cuda")] = 3e4   # what fp32 sums of squares lose the others beside
+    w = 1 + 0.3 * torch.randn(d, generator=g, device="cuda")
+    return x.to(t), r.to(t) if name == "residual" else None, w.to(t)
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("unit", [False, True])
+@pytest.mark.parametrize("name", ["odd rows", "residual", "long", "dominant", "dominant long", "narrow"])
+def test_norm_is_the_64_bit_norm_rounded_once(ssa, name, unit, t):
+    """The sums of up to 16384 squares, here and in the test, are each off by 2^14 * 2^-53 at most, halved by the root, and a handful of roundings of
+    2^-53 follow: 2^-38 covers both.  An element may part from the exact row's only if that much moves it, or its block's scale, over a border."""
+    x, r, w = norm_case(name, t)
+    rows = ssa.rms_norm_f8(x, weight=w, residual=r, residual_out=None if r is None else torch.empty_like(r), eps=1e-6, unit=unit)
+    h = x.double() if r is None else (x.float() + r.float()).to(t).double()
+    y = h / torch.sqrt((h * h).mean(dim=1, keepdim=True) + 1e-6) * w.double()
+    if unit:
+        y = y / y.norm(dim=1, keepdim=True).clamp(min=1e-12)
+    y = y.cpu().numpy()
+    lo, hi = plain.round_rows(y * (1 - 2.0 ** -38)), plain.round_rows(y * (1 + 2.0 ** -38))
+    got = plain.values(rows.codes.view(torch.uint8).cpu().numpy(), rows.scales.cpu().numpy(), rows.d)
+    assert ((got == lo) | (got == hi)).all()
+    assert np.mean(lo != hi) < 1e-6   # (the borders leave the rest nothing to hide in)
