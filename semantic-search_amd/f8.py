@@ -6,7 +6,9 @@ or take an `F8Rows` as it is - for instance what `rms_norm_f8(..., unit=True)` m
 what the reference's embedder does in fp32 before it hands rows to FAISS (core/qwen3_vl_embedding.py:447-448).
 
 All calls work on tensors of a ROCm device, enqueue on its current torch stream, wait for nothing and may be captured into a
-graph; none of them records a gradient.  Argument errors raise ValueError or TypeError, errors of the engine RuntimeError.
+graph; none of them records a gradient.  What they write into counts as changed in place (a backward pass that saved it raises), must not
+require a gradient outside of torch.no_grad(), and may overlap an input only where that is said.  Argument errors raise ValueError or
+TypeError, errors of the engine RuntimeError.
 """
 from typing import Optional
 
@@ -24,6 +26,15 @@ def _blocks(d: int) -> int:
 
 # handle of the current torch stream of device i (the Stream object around it costs more than a launch)
 _stream = torch._C._cuda_getCurrentRawStream
+
+
+# autograd's notice that a tensor has been written through its pointer
+_changed = torch.autograd.graph.increment_version
+
+
+def _writable(t: torch.Tensor, what: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} is written without a gradient but requires one: detach it, or call under torch.no_grad()")
 
 
 def _rows_arg(x, what: str) -> torch.Tensor:
@@ -132,6 +143,10 @@ class F8Rows:
         return out
 
 
+def _rows_changed(out: F8Rows) -> None:
+    _changed(out._buffer if out._buffer is not None else (out._codes, out._scales))
+
+
 def _out_rows(out: Optional[F8Rows], n: int, d: int, device_index: int, what: str) -> F8Rows:
     if out is None:
         return F8Rows.empty(n, d, device_index)
@@ -145,16 +160,19 @@ def quantize_f8(x: torch.Tensor, out: Optional[F8Rows] = None) -> F8Rows:
     x = _rows_arg(x, "quantize_f8")
     n, d = x.shape
     i = x.get_device()
-    out = _out_rows(out, n, d, i, "quantize_f8")
-    _lib.check(_lib.load().ssmi_f8_quantize(i, n, d, x.data_ptr(), _SRC[x.dtype], _stride(x), *out._args, _stream(i)))
-    return out
+    rows = _out_rows(out, n, d, i, "quantize_f8")
+    _lib.check(_lib.load().ssmi_f8_quantize(i, n, d, x.data_ptr(), _SRC[x.dtype], _stride(x), *rows._args, _stream(i)))
+    if out is not None:
+        _rows_changed(rows)
+    return rows
 
 
 def rms_norm_f8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                 residual_out: Optional[torch.Tensor] = None, eps: float = 1e-6, unit: bool = False, out: Optional[F8Rows] = None) -> F8Rows:
     """8-bit rows of the root-mean-square norm of h = x + residual: h / sqrt(mean(h^2) + eps) * weight, in 64 bits.
 
-    The sum is rounded to x's type and stored in `residual_out` (default: back into `residual`).  unit=True: rows of unit length,
+    The sum is rounded to x's type and stored in `residual_out` (default: back into `residual`; it may be `x` or `residual`, and else shares no
+    memory with them).  unit=True: rows of unit length,
     ready for an inner-product index."""
     x = _rows_arg(x, "rms_norm_f8")
     n, d = x.shape
@@ -174,16 +192,21 @@ def rms_norm_f8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual
                 raise ValueError(f"rms_norm_f8: {name} must be like x: shape {tuple(x.shape)}, {x.dtype}, {x.device}")
         if d > 1 and ro.stride(1) != 1 or n > 1 and ro.stride(0) < d:
             raise ValueError("rms_norm_f8: residual_out must have contiguous rows")
+        _writable(ro, "rms_norm_f8: residual" if residual_out is None else "rms_norm_f8: residual_out")
         if d > 1 and r.stride(1) != 1 or n > 1 and r.stride(0) < d:
             r = r.contiguous()
     elif residual_out is not None:
         raise ValueError("rms_norm_f8: residual_out without a residual")
-    out = _out_rows(out, n, d, i, "rms_norm_f8")
+    rows = _out_rows(out, n, d, i, "rms_norm_f8")
     _lib.check(_lib.load().ssmi_f8_rms_norm(
         i, n, d, x.data_ptr(), _SRC[x.dtype], _stride(x), r.data_ptr() if r is not None else None, _stride(r) if r is not None else 0,
         ro.data_ptr() if ro is not None else None, _stride(ro) if ro is not None else 0, w.data_ptr() if w is not None else None,
-        _SRC[w.dtype] if w is not None else 0, float(eps), 1 if unit else 0, *out._args, _stream(i)))
-    return out
+        _SRC[w.dtype] if w is not None else 0, float(eps), 1 if unit else 0, *rows._args, _stream(i)))
+    if ro is not None:
+        _changed(ro)
+    if out is not None:
+        _rows_changed(rows)
+    return rows
 
 
 def matmul_f8(a: F8Rows, b: F8Rows, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -201,10 +224,15 @@ def matmul_f8(a: F8Rows, b: F8Rows, out_dtype: torch.dtype = torch.bfloat16, out
         out_dtype = out.dtype
     if out_dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"matmul_f8: the output is float16 or bfloat16, not {out_dtype}")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((a.n, b.n), dtype=out_dtype, device=i)
     elif out.shape != (a.n, b.n) or out.get_device() != i or (b.n > 1 and out.stride(1) != 1) or (a.n > 1 and out.stride(0) < b.n):
         raise ValueError(f"matmul_f8: out must be ({a.n}, {b.n}) with contiguous rows on {a.device}")
+    else:
+        _writable(out, "matmul_f8: out")
     _lib.check(_lib.load().ssmi_f8_matmul(i, a.n, b.n, a.d, *a._args, *b._args, out.data_ptr(), _SRC[out_dtype],
                                           out.stride(0) if a.n > 1 else b.n, _stream(i)))
+    if given:
+        _changed(out)
     return out
