@@ -54,13 +54,36 @@ def _stride(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+def _layout_error(codes, scales, d: int) -> Optional[str]:
+    """What keeps the kernels from reading the tensors as rows of d elements, or None."""
+    for t, name, dtype in ((codes, "codes", torch.float8_e4m3fn), (scales, "scales", torch.uint8)):
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != 2:
+            return f"{name} must be a 2-D tensor of {dtype}"
+    ld, ls = _blocks(d) * BLOCK, (_blocks(d) + 3) // 4 * 4
+    if d < 1 or codes.shape[1] != ld or scales.shape[1] < ls or codes.shape[0] != scales.shape[0] or codes.device != scales.device:
+        return f"{d} elements need {ld} codes and {ls} scales a row, as many rows of both on one device, got {tuple(codes.shape)} and {tuple(scales.shape)}"
+    for t, name, width, unit in ((codes, "codes", ld, 16), (scales, "scales", ls, 4)):
+        if t.stride(1) != 1 or t.data_ptr() % unit or (t.shape[0] > 1 and (t.stride(0) % unit or t.stride(0) < width)):
+            return f"rows of {name} must be contiguous, {unit}-byte aligned and a multiple of {unit} bytes apart"
+    return None
+
+
 class F8Rows:
     """n rows of d elements in 8 bits: `codes` (n, whole blocks of 128) float8_e4m3fn, `scales` (n, >= blocks) uint8."""
 
     __slots__ = ("n", "d", "device_index", "_args", "_buffer", "_codes", "_scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, d: int):
-        self.n, self.d, self._codes, self._scales, self._buffer = codes.shape[0], int(d), codes, scales, None
+        """The tensors as they are, in the layout that the kernels read: rows of whole blocks of codes, zero behind d, and of scales in words of
+        four; `from_parts` takes others."""
+        d = int(d)
+        what = _layout_error(codes, scales, d)
+        if what:
+            raise ValueError(f"F8Rows: {what}")
+        self._set(codes, scales, d)
+
+    def _set(self, codes: torch.Tensor, scales: torch.Tensor, d: int) -> None:
+        self.n, self.d, self._codes, self._scales, self._buffer = codes.shape[0], d, codes, scales, None
         self.device_index = codes.get_device()
         # codes, their stride, scales, their stride: as the C entry points take them
         self._args = (codes.data_ptr(), codes.stride(0) if self.n > 1 else codes.shape[1],
@@ -131,7 +154,9 @@ class F8Rows:
         """A contiguous range of the rows (a view)."""
         if not isinstance(rows, slice) or rows.step not in (None, 1):
             raise TypeError("F8Rows: only plain slices of rows")
-        return F8Rows(self.codes[rows], self.scales[rows], self.d)
+        part = F8Rows.__new__(F8Rows)
+        part._set(self.codes[rows], self.scales[rows], self.d)   # (the layout is its whole's)
+        return part
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the rows stand for, (n, d); exact in float32 and bfloat16 (four significant bits times a power of two)."""
