@@ -118,8 +118,8 @@ class F8Rows:
 
     @classmethod
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, d: Optional[int] = None) -> "F8Rows":
-        """Rows from codes (n, d or whole blocks; float8_e4m3fn or uint8) and scale exponents (n, blocks; uint8).  The tensors
-        are used as they are where their layout allows; codes behind d are set to zero."""
+        """Rows from codes (n, d or whole blocks; float8_e4m3fn or uint8) and scale exponents (n, blocks; uint8).  The tensors are used as they are
+        where their layout allows and are never written; whole blocks whose codes behind d are not all zero are copied (to look waits for them)."""
         if codes.dim() != 2 or scales.dim() != 2 or codes.shape[0] != scales.shape[0]:
             raise ValueError(f"F8Rows: expected 2-D codes and scales of as many rows, got {tuple(codes.shape)} and {tuple(scales.shape)}")
         if not codes.is_cuda or codes.device != scales.device:
@@ -130,13 +130,14 @@ class F8Rows:
         blocks = _blocks(d)
         if d < 1 or codes.shape[1] not in (d, blocks * BLOCK) or scales.shape[1] < blocks:
             raise ValueError(f"F8Rows: {d} elements need {d} or {blocks * BLOCK} codes and {blocks} scales a row, got {codes.shape[1]} and {scales.shape[1]}")
-        raw = codes.view(torch.uint8)
-        if raw.shape[1] != blocks * BLOCK or raw.stride(1) != 1 or raw.stride(0) % 16 or raw.data_ptr() % 16 or raw.stride(0) < blocks * BLOCK:
-            fresh = torch.zeros((raw.shape[0], blocks * BLOCK), dtype=torch.uint8, device=raw.device)
+        raw, whole = codes.view(torch.uint8), blocks * BLOCK
+        copy = raw.shape[1] != whole or raw.stride(1) != 1 or raw.stride(0) % 16 or raw.data_ptr() % 16 or raw.stride(0) < whole
+        if not copy and d < whole:   # (a stream that is captured cannot be waited for)
+            copy = torch.cuda.is_current_stream_capturing() or bool((raw[:, d:] & 0x7F).any())
+        if copy:
+            fresh = torch.zeros((raw.shape[0], whole), dtype=torch.uint8, device=raw.device)
             fresh[:, :d] = raw[:, :d]
             raw = fresh
-        elif d < blocks * BLOCK:
-            raw[:, d:].zero_()
         if scales.stride(1) != 1 or scales.stride(0) % 4 or scales.data_ptr() % 4 or min(scales.shape[1], scales.stride(0)) < (blocks + 3) // 4 * 4:
             fresh = torch.zeros((scales.shape[0], (blocks + 3) // 4 * 4), dtype=torch.uint8, device=scales.device)
             fresh[:, :blocks] = scales[:, :blocks]
