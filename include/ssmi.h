@@ -198,11 +198,12 @@ int ssmi_index_write_append(ssmi_index* h, const char* path);
 int ssmi_index_read(const char* path, int storage_dtype, int device, ssmi_index** out);
 
 /* ---- 8-bit rows --------------------------------------------------------- */
-/* What feeds an index of SSMI_F8 storage, and the product it is built on (no reference counterpart: its embedder ends in a
+/* What feeds an index of SSMI_F8 storage, and the product of such rows (no reference counterpart: its embedder ends in a
  * root-mean-square norm and F.normalize, core/qwen3_vl_embedding.py:447-448, and hands fp32 rows to FAISS).  All pointers are
  * DEVICE memory of `device`; work is enqueued on `stream` (NULL = the HIP null stream), nothing is allocated or waited for,
  * so the calls may be captured into a graph.  Code rows: 16-byte aligned, codes_stride a multiple of 16 bytes >= SSMI_F8_LD(d);
- * scale rows: 4-byte aligned and readable to a multiple of 4 bytes, scales_stride a multiple of 4 bytes >= SSMI_F8_BLOCKS(d).  Strides of plain rows are in
+ * scale rows: 4-byte aligned and readable to a multiple of 4 bytes, scales_stride a multiple of 4 bytes >= SSMI_F8_BLOCKS(d).  Codes behind d are written as
+ * zeros and have to be zero (either sign) where rows are read, but for ssmi_index_add_f8, which keeps none.  Strides of plain rows are in
  * elements.  Outputs must not overlap inputs, unless stated. */
 /* (n, d) rows of src_dtype (SSMI_F32 / F16 / BF16) -> 8-bit rows; the codes behind d are written as zeros */
 int ssmi_f8_quantize(int device, int64_t n, int d, const void* x, int src_dtype, int64_t x_stride, uint8_t* codes,
@@ -223,8 +224,8 @@ int ssmi_f8_rms_norm(int device, int64_t n, int d, const void* x, int dtype, int
 int ssmi_f8_matmul(int device, int64_t m, int64_t n, int k, const uint8_t* a_codes, int64_t a_stride, const uint8_t* a_scales,
                    int64_t a_scales_stride, const uint8_t* b_codes, int64_t b_stride, const uint8_t* b_scales,
                    int64_t b_scales_stride, void* out, int out_dtype, int64_t out_stride, void* stream);
-/* ssmi_index_add of rows that are 8-bit already (an index of SSMI_F8 storage; device memory of its GPU): kept bit for bit.
- * The caller's writes to them must have completed. */
+/* ssmi_index_add of rows that are 8-bit already (an index of SSMI_F8 storage; device memory of its GPU): their d codes and
+ * their scales are kept bit for bit.  The caller's writes to them must have completed. */
 int ssmi_index_add_f8(ssmi_index* h, int64_t n, const uint8_t* codes, int64_t codes_stride, const uint8_t* scales,
                       int64_t scales_stride);
 /* ssmi_index_search_min of queries that are 8-bit already (device buffers throughout; returns after enqueueing).  An index of

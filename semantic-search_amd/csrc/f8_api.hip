@@ -317,6 +317,8 @@ int ssmi_index_add_f8(ssmi_index* h, int64_t n, const uint8_t* codes, int64_t co
     const int ns = f8_blocks(h->rows.d);
     CHECK(for_segments(h, h->rows.nrows, n, [&](long long first, long long cnt, unsigned char* c, unsigned char* s, float* lengths) -> int {
         HIPCHECK(hipMemcpy2DAsync(c, h->rows.ld, codes + first * codes_stride, codes_stride, h->rows.ld, cnt, hipMemcpyDeviceToDevice, h->stream));
+        // (whole blocks, which copies fast; what the caller has behind the d codes is not part of the row)
+        if (h->rows.d < h->rows.ld) HIPCHECK(hipMemset2DAsync(c + h->rows.d, h->rows.ld, 0, h->rows.ld - h->rows.d, cnt, h->stream));
         HIPCHECK(hipMemcpy2DAsync(s, h->scales.ld, scales + first * scales_stride, scales_stride, ns, cnt, hipMemcpyDeviceToDevice, h->stream));
         HIPCHECK(launch_f8_lengths(F8Mat{c, h->rows.ld, s, h->scales.ld, cnt}, h->rows.ld, lengths, (unsigned*)h->f8_longest, h->num_cu, h->stream));
         return 0;

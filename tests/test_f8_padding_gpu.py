@@ -47,3 +47,29 @@ def test_rows_from_parts_while_a_graph_is_captured(ssa):
         g.replay()
         assert torch.equal(out, want)
         torch.cuda.synchronize()
+
+
+def index_of(ssa, d, rows, dirty):
+    """An index whose rows came through the C entry point with codes behind them."""
+    from semantic_search_amd import _lib
+    index = ssa.IndexFlatIP(d, storage="f8")
+    scales = rows.scales.contiguous()
+    torch.cuda.synchronize()
+    _lib.check(_lib.load().ssmi_index_add_f8(index._handle(), len(rows), dirty.data_ptr(), dirty.stride(0), scales.data_ptr(), scales.stride(0)))
+    return index
+
+
+@pytest.mark.parametrize("d", [1, 100, 200, 300])
+def test_an_index_does_not_keep_codes_behind_its_rows(ssa, d, monkeypatch):
+    monkeypatch.setenv("SSMI_SEG_SHIFT", "8")
+    rows, dirty = padded(ssa, 700, d, 5)
+    before = dirty.clone()
+    index = index_of(ssa, d, rows, dirty)
+    assert torch.equal(dirty, before)
+    X = plain.values(rows.codes.view(torch.uint8).cpu().numpy(), rows.scales.cpu().numpy(), d)
+    for nq in (1, 5, 60, 300):
+        queries, dirty_q = padded(ssa, nq, d, 6 + nq)
+        Q = plain.values(queries.codes.view(torch.uint8).cpu().numpy(), queries.scales.cpu().numpy(), d)
+        want = plain.search(X, Q, 9)[1]
+        assert np.array_equal(index.search(queries, 9)[1].cpu().numpy(), want)
+        assert np.array_equal(index.search(ssa.F8Rows.from_parts(dirty_q, queries.scales, d), 9)[1].cpu().numpy(), want)
