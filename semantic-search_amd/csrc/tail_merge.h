@@ -20,7 +20,8 @@
 // barrier behind the ticket.  This is the guide's "sc1 stores + drained counter add + sc1 loads" hand-off (one
 // lane of each storing workgroup adds to ONE counter, the workgroup whose add came last reads).  All three are
 // properties of the generated instructions, so tools/check_tail_merge.py asserts them on the assembly of every
-// kernel with a tail (tests/test_tail_merge_isa_cpu.py), and tools/soak_tail_merge.py soaks the behaviour.
+// kernel with a tail (tests/test_tail_merge_isa_cpu.py; the built objects: tests/test_tail_merge_built_cpu.py), and tools/soak_tail_merge.py
+// soaks the behaviour.
 //
 // Stands in for the heap merge inside faiss.IndexFlatIP.search / IndexIVFFlat.search
 // (reference call site core/index_manager.py:371).
