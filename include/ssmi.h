@@ -231,9 +231,10 @@ int ssmi_index_add_f8(ssmi_index* h, int64_t n, const uint8_t* codes, int64_t co
 /* ssmi_index_search_min of queries that are 8-bit already (device buffers throughout; returns after enqueueing).  An index of
  * SSMI_F8 storage quantises fp32 queries by ssmi_f8_quantize, so both calls give the same results.  The answer is the k best rows by
  * the inner products of the 8-bit query with the 8-bit rows summed in 64 bits (rounded once to fp32; equal sums: the lower id first), in
- * any batch.  It is found among k + 16 candidates by fp32 sums; a query whose candidates are not proven to hold it - more than 16 rows within the
- * error of such sums, about 1e-5 |q||x|, of the k-th score, as copies of a row are - has all rows in question summed in 64 bits, up to
- * 1.4 ms over 1M x 4096.  NaN scores are never reported.
+ * any batch.  It is found among k + 16 candidates by the matrix cores' sums; a query whose candidates are not proven to hold it - more than 16
+ * rows within the error of such sums, about 1e-5 |q||x|, of the k-th score - has the rows in question summed in 64 bits: some hundred where
+ * a channel is much stronger than the others, all of them where copies of a row share the k-th place (0.8 ms a query over 1M x 4096).  NaN
+ * scores are never reported.
  * k <= 1008 (the other searches of such an index too). */
 int ssmi_index_search_f8(ssmi_index* h, int64_t nq, const uint8_t* codes, int64_t codes_stride, const uint8_t* scales,
                          int64_t scales_stride, int k, float min_score, float* D, int64_t* I, int64_t id_offset, void* stream);

@@ -18,7 +18,9 @@ namespace ssmi {
 static constexpr int kF8 = 3;             // SSMI_F8
 static constexpr int kF8Block = 128;      // codes per scale
 static constexpr int kF8Spare = 16;       // candidates beyond k that a search scores again in 64 bits
+static constexpr int kF8Collect = 2048;   // rows that a query's fp32 sums may leave in question before all rows are
 static constexpr int kF8Batch = 4096;     // queries of a search that travel together
+enum { kF8Fp32, kF8Scaled, kF8Again };
 static constexpr int kF8MaxNorm = 16384;  // elements of a row that the norm keeps in registers
 static constexpr int kF8MaxK = kMaxK - kF8Spare;
 
@@ -64,29 +66,33 @@ hipError_t launch_f8_score_rows(const F8View& v, const int64_t* ids, long long n
 // out[i][j] = <a_i, b_j>, (a.n, b.n) of out_dtype (SSMI_F16 / SSMI_BF16), row stride in elements
 hipError_t launch_f8_matmul(const F8Mat& a, const F8Mat& b, int k, void* out, int out_dtype, long long out_stride, int num_cu, hipStream_t s);
 
-// the lengths of rows, rounded up (a row that holds a NaN: -1), and *longest (the bits of a positive float) = the largest of it and them
+// the lengths of rows, rounded up (a row that holds a NaN: -1); longest (the bits of positive floats): [0] the largest of it and them, [1] the same of
+// the lengths of the rows' largest elements, one of every eight neighbours (none less than 2^-6 of its block's scale)
 hipError_t launch_f8_lengths(const F8Mat& m, int ld, float* lengths, unsigned* longest, int num_cu, hipStream_t s);
 
 // What the second pass of a search leaves for the third.  ticket 0: the query is answered; else it counts the workgroups that are done with it,
-// from 1, and pos their entries.  No row with a score below edge is among the k best, nor one that is not on the list and shorter than `from`.
-struct F8State { double edge; float from; unsigned ticket, pos, unused; };
+// from 1, and pos their entries.  No row with a score below edge is among the k best, nor one that is not on the list and shorter than `from`,
+// nor one whose fp32 sum s and length x have s + slope x < least.  found: how many rows have not, more than kF8Collect: unknown
+struct F8State { double edge; float from, least, slope; unsigned ticket, pos, found; };
 struct F8Entry { double score; long long id; };
 
 // search over a row store: the k best of every query with their scores summed in 64 bits
 struct F8SearchPlan {
-    int kp;                   // candidates kept per query by the first pass: min(k + kF8Spare, kMaxK)
+    int kp;                   // candidates kept per query by the first pass
     int parts;                // partial lists per query
     bool scan;                // streaming scan (few queries), else the tile kernel
     int bt, r, threads, grid_x;
     int nb;                   // scan: blocks per row where that is 1, 2 or 4, 8 where it is a multiple of 8, else 0
     int cap, every;           // scan: candidates a query's buffer holds, turns of three stages between two looks at them
     int tq, nqt, nslices, gtop_m;
+    bool scaled;              // 256 queries a tile: the scaled instruction first, fp32 sums for the tiles with queries that those do not prove
     long long rows_per_slice;
     size_t lds, partial_bytes, cand_bytes, share_bytes;
     const char* kernel;
 };
 bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8SearchPlan* p);
-hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& p, void* share, void* cand, skey_t* partial, hipStream_t s);
+// open: not null for the second run of a scaled plan
+hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& p, const F8State* open, void* share, void* cand, skey_t* partial, hipStream_t s);
 // the streaming scan of up to p.bt queries, and what follows the first pass; queries: fp32 rows of d elements at f32, else q.codes
 struct F8ScanArgs {
     F8View v;
@@ -103,13 +109,17 @@ struct F8ScanArgs {
     int64_t id_offset;
     unsigned min_ord;
     int cap, every;
-    const float* longest;     // no row is longer
+    const float* longest;     // of launch_f8_lengths
+    int sums;                 // what the first pass added up with: kF8Fp32, kF8Scaled, or kF8Again: fp32 for the queries that state holds open
     F8State* state;           // [q.n], written by the second pass
+    unsigned char* open;      // [q.n][v.X.ld] codes, then [q.n][v.sld] scales: the queries it leaves; nullptr: for the exact pass as they are
+    unsigned* rows;           // [q.n][kF8Collect] the rows in question of each
     F8Entry* lists;           // [num_cu][k], of the exact pass
 };
 hipError_t launch_f8_scan(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s);
 hipError_t launch_f8_finish(const F8ScanArgs& a, const F8SearchPlan& p, hipStream_t s);
-// the queries whose lists the second pass could not prove, over all rows in 64 bits
+// the queries whose lists the second pass could not prove: rows in question by fp32 sums, and those, or all, in 64 bits
+hipError_t launch_f8_collect(const F8ScanArgs& a, int num_cu, hipStream_t s);
 hipError_t launch_f8_exact(const F8ScanArgs& a, int num_cu, hipStream_t s);
 
 #ifdef __HIPCC__

@@ -137,7 +137,7 @@ hipError_t gather_store_rows(ssmi_index* h, const RowStore& R, long long view_ro
     return launch_gather_rows(v, R.dtype, ids, n, R.d, out, bad, s);
 }
 
-// Workspaces: 4 query codes and scales, 5 candidate buffers, 2 partial lists, 6 states and lists of the exact pass, 7 shared thresholds.
+// Workspaces: 4 query codes and scales, 5 candidate buffers, 2 partial lists, 6 states, rows in question, open queries and lists of the exact pass, 7 shared thresholds.
 int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float* Ddev, int64_t* Idev, int64_t id_offset, hipStream_t s,
                     unsigned min_ord) {
     const RowStore& R = h->rows;
@@ -151,7 +151,9 @@ int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float*
         if (!plan_f8_search(ld, R.nrows, nb, k, h->num_cu, &p)) return fail("internal: 8-bit search plan failed");
         const bool rec = h->timing_on && done == 0;
         CHECK(ensure_ws(h, 2, p.partial_bytes));
-        CHECK(ensure_ws(h, 6, (size_t)nb * sizeof(F8State) + (size_t)h->num_cu * k * sizeof(F8Entry)));
+        const bool collect = nb > 1;   // (one query: all rows in 64 bits take little longer, and the launch 3 us of every search)
+        const size_t states = (size_t)nb * sizeof(F8State), lists = (size_t)h->num_cu * k * sizeof(F8Entry), rows = (size_t)nb * kF8Collect * sizeof(unsigned);
+        CHECK(ensure_ws(h, 6, states + lists + (collect ? rows + (size_t)nb * (ld + sld) : 0)));
         F8ScanArgs a = {};
         a.v = view;
         a.q = F8Mat{q.codes + done * q.stride, q.stride, q.scales + done * q.sstride, q.sstride, nb};
@@ -171,6 +173,8 @@ int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float*
         a.longest = h->f8_longest;
         a.state = (F8State*)h->ws[6];
         a.lists = (F8Entry*)(a.state + nb);
+        a.rows = (unsigned*)(a.lists + (size_t)h->num_cu * k);
+        a.open = collect ? (unsigned char*)h->ws[6] + states + lists + rows : nullptr;
         if (p.scan) {
             if (h->tail_counters) {
                 a.counter = nb == 1 ? h->tail_counters : nullptr;
@@ -191,10 +195,17 @@ int f8_store_search(ssmi_index* h, int64_t nq, const F8Queries& q, int k, float*
             CHECK(ensure_ws(h, 5, p.cand_bytes));
             CHECK(ensure_ws(h, 7, p.share_bytes));
             if (rec) HIPCHECK(hipEventRecord(ev[0], s));
-            HIPCHECK(launch_f8_tiles(view, a.q, p, h->ws[7], h->ws[5], (skey_t*)h->ws[2], s));
+            HIPCHECK(launch_f8_tiles(view, a.q, p, nullptr, h->ws[7], h->ws[5], (skey_t*)h->ws[2], s));
+            if (p.scaled) {
+                a.sums = kF8Scaled;
+                HIPCHECK(launch_f8_finish(a, p, s));
+                a.sums = kF8Again;
+                HIPCHECK(launch_f8_tiles(view, a.q, p, a.state, h->ws[7], h->ws[5], (skey_t*)h->ws[2], s));
+            }
             if (rec) HIPCHECK(hipEventRecord(ev[1], s));
         }
         if (!a.counter) HIPCHECK(launch_f8_finish(a, p, s));
+        if (collect) HIPCHECK(launch_f8_collect(a, h->num_cu, s));
         HIPCHECK(launch_f8_exact(a, h->num_cu, s));
         if (rec) { HIPCHECK(hipEventRecord(ev[2], s)); h->merge_event = true; }
     }

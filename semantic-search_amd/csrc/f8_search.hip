@@ -1,14 +1,21 @@
 // f8_search.hip - Flat search over 8-bit rows (f8.h): the product of f8_tile.h with the top-k epilogues of the other row types.
 //
-// The answer is the k best rows by the exact sums: score descending, ties by the lower id.  Three passes.  The first keeps, for every query, the
-// best k + 16 rows by the matrix cores' fp32 sums: a streaming scan for a few queries, bound by reading the rows once (for one query
-// its launch carries the second pass), or the tile kernel with the candidate buffers of the 16-bit kernels (mfma_common.h).  The second sums those
-// candidates' products in 64 bits - every product of two codes is exact in fp32 and the scales are powers of two, so the sum is exact or off by a
-// rounding of 2^-53 - and sorts them by that.  It also proves the list: a row that is not on it has a first-pass sum of at most the last one's, and
-// an exact one that is higher by the first pass's error at most, which goes by the row's length.  A row that is too short to make up for the gap
-// between the k-th exact score and the last sum is not among the k best.  The third pass takes the queries that some row is long enough for - more
-// than 16 rows within some 1e-5 |q||x| of the k-th score, copies of a row above all, or rows far longer than the others - and
-// sums those rows in 64 bits.  A query therefore gets the same ids and scores in any batch.
+// The answer is the k best rows by the exact sums: score descending, ties by the lower id.
+//
+//   1. candidates   the best k + 16 rows by the matrix cores' sums: a streaming scan for a few queries, bound by reading the rows once (for one
+//                   query its launch carries step 2), or the tile kernels with the candidate buffers of the 16-bit kernels (mfma_common.h)
+//   2. proof        the candidates' products summed in 64 bits - every product of two codes is exact in fp32 and the scales are powers of two, so
+//                   a sum is exact or off by a rounding of 2^-53 - and sorted by that.  A row that is not among them has a sum of step 1 of at
+//                   most the last one's, and an exact one that is higher by that sum's error at most, which goes by the row's length.  If no row
+//                   is long enough to make up for the gap between the k-th exact score and the last sum, the list is the answer.
+//   3. in question  (not for one query) for the queries that are left - more than 16 rows within some 1e-5 |q||x| of the k-th score: a strong
+//                   channel that makes the sums coarse against the gaps, copies of a row, rows far longer than the others - the rows whose sum
+//                   may have lost enough for the k-th score
+//   4. exact        those rows, or every row that is long enough, in 64 bits
+//
+// Sums are fp32's (f8_tile.h), but for tiles of 256 queries and small k: there the scaled instruction's come first, with their own, larger error in step 2,
+// and steps 1 and 2 run again with fp32's for the tiles that hold an open query.  Steps that find nothing to do are a launch of 3 us each.  A
+// query gets the same ids and scores in any batch.
 //
 // Same place on the path as the 16-bit kernels: faiss.IndexFlatIP.search as called from core/index_manager.py:371.
 #include "f8_pp.h"
@@ -55,6 +62,27 @@ __device__ __forceinline__ float f8_from(int blocks, double q, double gap) {
     const double x = (gap - 0x1p-118 * q - 0x1p-125) / (f8_relative(blocks) * q + 0x1p-118);
     return x > 0.0 ? (float)(fmin(fmin(x, 1e37), 1e37 / fmax(q, 1e-300)) * (1 - 0x1p-20)) : 0.f;
 }
+// How far a sum of the scaled instruction may be off, where no sum leaves fp32: of eight neighbouring products it keeps the largest, p = 2^E f, and
+// takes the other seven down to multiples of 2^(E - 13); an exponent counts 2^-6 at the least (of subnormal codes, measured).  The largest products are
+// at most g h, element by element of the largest of the eights of q and x, and their sum at most |g||h|.  Adding the eights up costs it no more
+// than four times what the fp32 sums of all products may (random rows: a tenth of either).
+__device__ __forceinline__ double f8_scaled_error(int blocks, double q, double x, double g, double h) {
+    return 7.0 / 8192 * g * h + 4.0 * f8_relative(blocks) * q * x + 0x1p-100 * (1.0 + q + x);
+}
+// the squares of the largest of eight codes and of the eight behind them, added
+__device__ __forceinline__ float eights(const i32x4_t& x) {
+    float sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < 4; h += 2) {
+        float a[4], b[4], m = 0x1p-6f;
+        f8_unpack4((unsigned)x[h], a);
+        f8_unpack4((unsigned)x[h + 1], b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(fabsf(a[j]), fabsf(b[j])));
+        sum = fmaf(m, m, sum);   // (multiples of 2^-12 below 2^19: off by 2^-24 of itself at most)
+    }
+    return sum;
+}
 // a score of the sorted list; the score floor cuts a suffix of it
 __device__ __forceinline__ void put_result(const F8ScanArgs& A, float* D, int64_t* I, int rank, double s, int64_t id) {
     const float f = (float)s;
@@ -63,7 +91,7 @@ __device__ __forceinline__ void put_result(const F8ScanArgs& A, float* D, int64_
     I[rank] = keep ? id + A.id_offset : -1;
 }
 // the LDS words that a query's second pass needs besides its sort: kp scores, kp ids of its own and kp that it is given, then these
-struct F8Proof { double qq, kth; skey_t last; };   // |q|^2, the k-th exact score, the last key of a full list (else 0)
+struct F8Proof { double qq, gg, kth; skey_t last; };   // |q|^2, that of the eights' largest, the k-th exact score, the last key of a full list (else 0)
 __host__ __device__ inline size_t finish_bytes(int kp) { return (size_t)kp * 24 + sizeof(F8Proof); }
 struct F8Scratch {
     double* score;
@@ -82,15 +110,16 @@ __device__ __forceinline__ void finish_query(const F8ScanArgs& A, long long qi, 
     float* D = A.D + qi * k;
     int64_t* I = A.I + qi * k;
     if (wave == nwaves - 1) {
-        double qq = 0.0;
+        double qq = 0.0, gg = 0.0;
         for (int e = lane * 16; e < V.X.ld; e += 1024) {
             const i32x4_t y = *reinterpret_cast<const i32x4_t*>(qc + e);
             const double sq = (double)f8_scale(qsc[e / kF8Block]);
             qq += dot16(y, y) * (sq * sq);
+            gg += (double)eights(y) * (sq * sq);
         }
 #pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) qq += __shfl_xor(qq, d);
-        if (lane == 0) L.proof->qq = qq;
+        for (int d = 32; d >= 1; d >>= 1) { qq += __shfl_xor(qq, d); gg += __shfl_xor(gg, d); }
+        if (lane == 0) { L.proof->qq = qq; L.proof->gg = gg; }
     }
     const long long seg_mask = (1ll << V.X.seg_shift) - 1;
     for (int c0 = wave * N; c0 < kp; c0 += nwaves * N) {
@@ -158,9 +187,23 @@ __device__ __forceinline__ void finish_query(const F8ScanArgs& A, long long qi, 
         // The list may lack a row whose sum came out at its last one's or below (a list that is not full: only one that left fp32).  Such a row is
         // among the k best only if it gained the gap.  (A query that is NaN has no results.)
         const double gap = p.last == 0 ? __builtin_inf() : valid >= k ? p.kth - (double)key_score(p.last) : -__builtin_inf();
-        const float from = f8_from(V.X.ld / kF8Block, sqrt(p.qq) * (1 + 0x1p-40), gap);
-        const bool proven = p.qq != p.qq || *A.longest < from;
-        A.state[qi] = F8State{valid >= k ? p.kth : -__builtin_inf(), from, proven ? 0u : 1u, 0u, 0u};
+        const double q = sqrt(p.qq) * (1 + 0x1p-40);
+        const float from = f8_from(V.X.ld / kF8Block, q, gap);
+        bool proven = p.qq != p.qq || A.longest[0] < from;
+        if (A.sums == kF8Scaled && proven && p.qq == p.qq)
+            proven = gap > f8_scaled_error(V.X.ld / kF8Block, q, (double)A.longest[0], sqrt(p.gg) * (1 + 0x1p-20), (double)A.longest[1]);
+        const double x = (double)A.longest[0];
+        const bool sums = valid >= k && p.last != 0 && q < 1e37 && x < 1e37 && q * x < 1e37;   // no sum leaves fp32
+        // (rounded outwards, and the sum that is compared with it is off by 2^-24 of itself)
+        const float least = (float)(p.kth - fabs(p.kth) * 0x1p-22 - 0x1p-118 * (q + x) - 0x1p-125), slope = (float)(f8_relative(V.X.ld / kF8Block) * q * (1 + 0x1p-20));
+        A.state[qi] = F8State{valid >= k ? p.kth : -__builtin_inf(), from, sums ? least : 0.f, sums ? slope : 0.f, proven ? 0u : 1u, 0u, sums && A.open ? 0u : kF8Collect + 1u};
+        L.proof->last = proven || A.sums == kF8Scaled || !A.open ? 0 : 1;
+    }
+    __syncthreads();
+    if (L.proof->last) {   // the collecting pass reads it from there
+        for (int e = threadIdx.x * 16; e < V.X.ld; e += blockDim.x * 16)
+            *reinterpret_cast<i32x4_t*>(A.open + qi * V.X.ld + e) = *reinterpret_cast<const i32x4_t*>(qc + e);
+        for (int b = threadIdx.x; b < V.X.ld / kF8Block; b += blockDim.x) A.open[A.q.n * V.X.ld + qi * V.sld + b] = qsc[b];
     }
 }
 
@@ -297,6 +340,7 @@ __global__ void __launch_bounds__(1024) f8_finish_kernel(F8ScanArgs A, int P) {
     extern __shared__ __align__(16) unsigned char smem[];
     const long long qi = blockIdx.x;
     const int ld = A.v.X.ld, kp = A.kp;
+    if (A.sums == kF8Again && A.state[qi].ticket == 0) return;   // proven
     unsigned char* qs = smem;
     unsigned char* qsc = smem + ld;
     skey_t* keys = reinterpret_cast<skey_t*>(smem + (ld + ld / kF8Block + 15) / 16 * 16);
@@ -307,9 +351,29 @@ __global__ void __launch_bounds__(1024) f8_finish_kernel(F8ScanArgs A, int P) {
     finish_query(A, qi, qs, qsc, L);
 }
 
-// ---- third pass: the queries that are not proven, over all rows.  A workgroup per CU ----
-// Scores as finish_query's.  W workgroups share a query (all of the grid if it is alone), each takes a range of the rows, picks those that are
-// long enough and keeps what may be among the k best in LDS, sorted down to k whenever the buffer fills; the last to finish joins their lists.  1M x 4096 with every row long enough: 1.4 ms
+// ---- third pass: the queries that are not proven.  A workgroup per CU ----
+// their numbers: from the front of list those that are to see all rows (n[0] of them), from the back the others (n[1]).  All threads
+__device__ __forceinline__ void open_queries(const F8ScanArgs& A, unsigned short* list, unsigned* n) {
+    const int lane = lane_id(), nq = (int)A.q.n;
+    if (threadIdx.x < 64) {
+        int all = 0, few = 0;
+        for (int q0 = 0; q0 < nq; q0 += 64) {
+            const F8State* st = A.state + min(q0 + lane, nq - 1);
+            const bool is = q0 + lane < nq && __hip_atomic_load(&st->ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
+            const bool whole = is && st->found > (unsigned)kF8Collect;
+            const unsigned long long ma = __builtin_amdgcn_ballot_w64(whole), mf = __builtin_amdgcn_ballot_w64(is && !whole), below = (1ull << lane) - 1;
+            if (whole) list[all + __builtin_popcountll(ma & below)] = (unsigned short)(q0 + lane);
+            else if (is) list[kF8Batch - 1 - few - __builtin_popcountll(mf & below)] = (unsigned short)(q0 + lane);
+            all += __builtin_popcountll(ma);
+            few += __builtin_popcountll(mf);
+        }
+        if (lane == 0) { n[0] = (unsigned)all; n[1] = (unsigned)few; }
+    }
+    __syncthreads();
+}
+
+// Scores as finish_query's.  A query whose rows in question are known has a workgroup score those.  Of the others, W workgroups share one (all of the
+// grid if it is alone); each takes a range of the rows, picks those that are long enough and keeps what may be among the k best in LDS, sorted down to k whenever the buffer fills; the last to finish joins their lists.  1M x 4096 with every row long enough: 1.4 ms
 // for one query, 0.8 ms for each of many, by the vector units (four instructions a product).  With nothing to do the launch costs 3 us.
 static constexpr int kExactThreads = 1024, kExactEntries = 2048, kExactRound = 256;   // entries of a buffer, and how many a round may add
 struct F8Exact {
@@ -371,25 +435,16 @@ __global__ void __launch_bounds__(kExactThreads) f8_exact_kernel(F8ScanArgs A) {
     unsigned* sel = reinterpret_cast<unsigned*>(open + kF8Batch);            // [blockDim.x] rows of a round
     unsigned char* qs = reinterpret_cast<unsigned char*>(sel + blockDim.x);
     unsigned char* qsc = qs + ld;
-    if (wave == 0) {
-        int n = 0;
-        for (int q0 = 0; q0 < nq; q0 += 64) {
-            const bool is = q0 + lane < nq && __hip_atomic_load(&A.state[q0 + lane].ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
-            const unsigned long long m = __builtin_amdgcn_ballot_w64(is);
-            if (is) open[n + __builtin_popcountll(m & ((1ull << lane) - 1))] = (unsigned short)(q0 + lane);
-            n += __builtin_popcountll(m);
-        }
-        if (lane == 0) X.count[1] = (unsigned)n;
-    }
-    __syncthreads();
-    const int nopen = (int)X.count[1];
-    if (nopen == 0) return;
-    const int W = max(1, (int)gridDim.x / nopen);
+    open_queries(A, open, X.count + 1);
+    const int nall = __builtin_amdgcn_readfirstlane((int)X.count[1]), nfew = __builtin_amdgcn_readfirstlane((int)X.count[2]);
+    if (nall + nfew == 0) return;
+    const int W = nall ? max(1, (int)gridDim.x / nall) : 1;
     // lanes that share a row: 16 codes each, added up in finish_query's order, so that a row has one score
     const int lpr = ld > 512 ? 64 : ld > 256 ? 32 : ld > 128 ? 16 : 8, rpw = 64 / lpr, sub = lane / lpr, off = (lane % lpr) * 16;
     const long long seg_mask = (1ll << V.X.seg_shift) - 1;
-    for (int item = blockIdx.x; item < nopen * W; item += gridDim.x) {
-        const int u = item / W, part = item % W;
+    for (int item = blockIdx.x; item < nall * W + nfew; item += gridDim.x) {
+        const bool all = item < nall * W;
+        const int u = all ? item / W : kF8Batch - 1 - (item - nall * W), part = all ? item % W : 0;
         const long long qi = open[u];
         float* D = A.D + qi * k;
         int64_t* I = A.I + qi * k;
@@ -400,15 +455,16 @@ __global__ void __launch_bounds__(kExactThreads) f8_exact_kernel(F8ScanArgs A) {
         X.thr_id = 0xffffffffu;
         __syncthreads();
         const float from = A.state[qi].from;
-        const long long begin = V.X.nrows * part / W, end = V.X.nrows * (part + 1) / W;
-        for (long long r0 = part == 0 ? begin - (long long)blockDim.x : begin; r0 < end; r0 += blockDim.x) {
-            // the rows that are long enough (a NaN's -1 is not), and before them the second pass's results that are not
+        const unsigned* rows = A.rows + qi * kF8Collect;
+        const long long begin = all ? V.X.nrows * part / W : 0, end = all ? V.X.nrows * (part + 1) / W : (long long)A.state[qi].found;
+        for (long long r0 = all && part == 0 ? begin - (long long)blockDim.x : begin; r0 < end; r0 += blockDim.x) {
+            // all: the rows that are long enough (a NaN's -1 is not), and before them the second pass's results that are not
             const bool listed = r0 < begin;
             const int e = threadIdx.x;
             if (listed ? e < k && !(I[e] == -1 && D[e] == SSMI_NEG_MAX) : r0 + e < end) {
-                const long long row = listed ? I[e] - A.id_offset : r0 + e;
-                const float len = static_cast<const float*>(V.lsegs[row >> V.X.seg_shift])[row & seg_mask];
-                if ((len >= from) != listed) sel[atomicAdd(X.count + 1, 1u)] = (unsigned)row;
+                const long long row = listed ? I[e] - A.id_offset : all ? r0 + e : (long long)rows[r0 + e];
+                const float len = all ? static_cast<const float*>(V.lsegs[row >> V.X.seg_shift])[row & seg_mask] : 0.f;
+                if (!all || (len >= from) != listed) sel[atomicAdd(X.count + 1, 1u)] = (unsigned)row;
             }
             __syncthreads();
             const int nsel = (int)X.count[1];
@@ -433,7 +489,7 @@ __global__ void __launch_bounds__(kExactThreads) f8_exact_kernel(F8ScanArgs A) {
             __syncthreads();
         }
         int n = X.shrink(k);
-        if (W > 1) {
+        if (all && W > 1) {
             // (A.lists: W k entries for each of the queries, filled by whoever is done)
             F8Entry* list = A.lists + (size_t)u * W * k;
             F8State* st = A.state + qi;
@@ -445,7 +501,7 @@ __global__ void __launch_bounds__(kExactThreads) f8_exact_kernel(F8ScanArgs A) {
             __syncthreads();
             if (threadIdx.x == 0) X.count[1] = __hip_atomic_fetch_add(&st->ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
-            if (X.count[1] != (unsigned)W) return;   // (a grid with W > 1 has one item a workgroup)
+            if (X.count[1] != (unsigned)W) continue;
             __threadfence();
             const int total = (int)__hip_atomic_load(&st->pos, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (threadIdx.x == 0) X.count[0] = 0;
@@ -469,28 +525,100 @@ __global__ void __launch_bounds__(kExactThreads) f8_exact_kernel(F8ScanArgs A) {
     }
 }
 
+// ---- rows in question ----
+// The first pass again for the queries that it did not answer, with what is known now: a row whose fp32 sum cannot have lost enough for the k-th score
+// is out.  What is left - a hundred rows or two, where a strong channel makes the sums coarse against the gaps of the scores - the next
+// launch scores, and only a query with more than kF8Collect such rows (copies) has to see all.  256 rows x 64 of the open queries a step.
+// 1M x 4096, 1024 queries, 0.98 of every row in one channel, k = 100: 16.5 ms with the passes in front and behind (all rows in 64 bits: 852 ms).
+static constexpr int kCollectQueries = 64;
+using F8CollectTile = F8Tile<2, 4, 8, 1, 3>;
+__global__ void __launch_bounds__(512) f8_collect_kernel(F8ScanArgs A) {
+    using T = F8CollectTile;
+    static_assert(T::XR == 256 && T::QR == kCollectQueries, "rows of a segment, queries of a step");
+    extern __shared__ __align__(16) unsigned char smem[];
+    float* lens = reinterpret_cast<float*>(smem + T::LDS);                    // [256]
+    unsigned* count = reinterpret_cast<unsigned*>(lens + 256);                // [4]
+    unsigned short* open = reinterpret_cast<unsigned short*>(count + 4);      // [kF8Batch]
+    const F8View& V = A.v;
+    const int ld = V.X.ld;
+    open_queries(A, open, count);
+    const int nopen = __builtin_amdgcn_readfirstlane((int)count[1]);
+    if (nopen == 0) return;
+    T t;
+    t.init(smem, ld / kF8Block);
+    const int frow = t.lane & 15, fq = t.lane >> 4;
+    const long long seg_mask = (1ll << V.X.seg_shift) - 1;
+    const long long tiles = (V.X.nrows + 255) / 256;
+    const int nqt = (nopen + kCollectQueries - 1) / kCollectQueries, slices = (int)min(tiles, (long long)max(1, (int)gridDim.x / nqt));
+    for (int item = blockIdx.x; item < nqt * slices; item += gridDim.x) {
+        const int qt = item % nqt, slice = item / nqt, q0 = qt * kCollectQueries;
+        const auto query = [&](int r) __attribute__((always_inline)) { return (int)open[kF8Batch - 1 - (q0 + r)]; };
+        const F8Src q{A.open, A.open + A.q.n * ld, (unsigned)ld, (unsigned)V.sld, min(kCollectQueries, nopen - q0) - 1};
+        float least[4], slope[4];
+        int qi[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int r = (t.wn * 4 + n) * 16 + frow;
+            qi[n] = query(min(r, q.last));
+            least[n] = r <= q.last ? A.state[qi[n]].least : __builtin_inff();
+            slope[n] = A.state[qi[n]].slope;
+        }
+        for (long long tile = tiles * slice / slices; tile < tiles * (slice + 1) / slices; ++tile) {
+            const long long row0 = tile * 256, seg = row0 >> V.X.seg_shift, off = row0 & seg_mask;
+            const int last = (int)min(255ll, V.X.nrows - 1 - row0);
+            __syncthreads();   // the tile before is done with
+            if (threadIdx.x < 256) lens[threadIdx.x] = static_cast<const float*>(V.lsegs[seg])[off + min((int)threadIdx.x, last)];
+            __syncthreads();
+            t.aim(F8Src{static_cast<const unsigned char*>(V.X.segs[seg]) + off * ld, static_cast<const unsigned char*>(V.ssegs[seg]) + off * V.sld, (unsigned)ld, (unsigned)V.sld, last}, q, query);
+            f32x4_t acc[2][4];
+            zero_acc(acc);
+            t.run(acc);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const int r = (t.wm * 2 + m) * 16 + fq * 4;
+                const float4 len = *reinterpret_cast<const float4*>(lens + r);
+                const float l[4] = {len.x, len.y, len.z, len.w};
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (fmaf(slope[n], l[i], acc[m][n][i]) >= least[n] && r + i <= last) {   // (a NaN is not)
+                            const unsigned pos = atomicAdd(&A.state[qi[n]].found, 1u);
+                            if (pos < (unsigned)kF8Collect) A.rows[(long long)qi[n] * kF8Collect + pos] = (unsigned)(row0 + r + i);
+                            else least[n] = __builtin_inff();   // all rows, then: no need to count on
+                        }
+            }
+        }
+    }
+}
+
 // lengths of rows: the waves take groups of rows as above
 __global__ void __launch_bounds__(256) f8_lengths_kernel(F8Mat m, int ld, float* lengths, unsigned* longest) {
     const int lane = lane_id(), wave = threadIdx.x >> 6;
     const int lpr = ld > 512 ? 64 : ld > 256 ? 32 : ld > 128 ? 16 : 8, rpw = 64 / lpr, sub = lane / lpr, off = (lane % lpr) * 16;
-    float most = 0.f;
+    float most = 0.f, most8 = 0.f;
     for (long long r0 = ((long long)blockIdx.x * 4 + wave) * rpw; r0 < m.n; r0 += (long long)gridDim.x * 4 * rpw) {
         const long long row = min(r0 + sub, m.n - 1);
-        double sum = 0.0;
+        double sum = 0.0, sum8 = 0.0;
 #pragma unroll 2
         for (int e = off; e < ld; e += lpr * 16) {
             const i32x4_t x = *reinterpret_cast<const i32x4_t*>(m.codes + row * m.stride + e);
             const double s = (double)f8_scale(m.scales[row * m.sstride + e / kF8Block]);
             sum += dot16(x, x) * (s * s);
+            sum8 += (double)eights(x) * (s * s);
         }
-        for (int d = lpr >> 1; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
+        for (int d = lpr >> 1; d >= 1; d >>= 1) { sum += __shfl_xor(sum, d); sum8 += __shfl_xor(sum8, d); }
         const float len = sum >= 0.0 ? (float)(sqrt(sum) * (1 + 0x1p-22)) : -1.f;   // (beyond fp32: infinite)
         if (off == 0 && r0 + sub < m.n) lengths[row] = len;
         most = fmaxf(most, len);
+        if (len >= 0.f) most8 = fmaxf(most8, (float)(sqrt(sum8) * (1 + 0x1p-20)));
     }
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-    if (lane == 0 && most > 0.f) atomicMax(longest, __float_as_uint(most));
+    for (int d = 32; d >= 1; d >>= 1) { most = fmaxf(most, __shfl_xor(most, d)); most8 = fmaxf(most8, __shfl_xor(most8, d)); }
+    if (lane == 0) {
+        if (most > 0.f) atomicMax(longest, __float_as_uint(most));
+        if (most8 > 0.f) atomicMax(longest + 1, __float_as_uint(most8));
+    }
 }
 hipError_t launch_f8_lengths(const F8Mat& m, int ld, float* lengths, unsigned* longest, int num_cu, hipStream_t s) {
     if (m.n <= 0) return hipSuccess;
@@ -857,7 +985,7 @@ __global__ void __launch_bounds__(512) f8_search_tile_kernel(F8View V, F8Mat q, 
 // Threshold filter over a wave's 128 x 64 accumulators (acc[m][n][4 g + e]: row row_base + 32 m + 8 g + 4 h + e, query q_base + 32 n + r
 // of lane (r, h)): as filter_tile of the 16-bit kernels, one column maximum first, survivors one by one.
 template <bool FULL>
-__device__ __forceinline__ void filter_big(const F8Pp::Acc& acc, int row_base, int q_base, int lane, long long row0, int rows_valid, skey_t* cand,
+__device__ __forceinline__ void filter_big(const F8Pp<false>::Acc& acc, int row_base, int q_base, int lane, long long row0, int rows_valid, skey_t* cand,
                                            const float* thr_l, unsigned* cnt_l, unsigned* flag_l) {
     const int r = lane & 31, h = lane >> 5;
 #pragma unroll
@@ -899,21 +1027,24 @@ __device__ __forceinline__ void filter_big(const F8Pp::Acc& acc, int row_base, i
 
 // A workgroup keeps its query tile and walks a slice of the rows; the first slab of the next row tile travels under this one's filter.
 // Folds, thresholds and the bound from the slices' published tops are those of the 16-bit kernel (mfma_pp.hip).
-// 1M x 4096, 1024 queries: 6.65 ms, 1.26 PFLOP/s (1.55 for the product alone, f8_matmul.hip); 256 queries: 1.93 ms - one slab ahead of the
-// products does not cover the way from memory where no second query tile shares the rows.
-template <int R>
-__global__ void __launch_bounds__(512, 2) f8_search_big_kernel(F8View V, F8Mat q, MfmaParams P) {
+// 1M x 4096, 1024 queries, k = 10: 3.86 ms with the scaled instruction, 2.23 PFLOP/s; 6.65 with fp32 sums, 1.29 (1.55 for the product alone,
+// f8_matmul.hip).  256 queries: 1.34 and 1.93 ms - one slab ahead of the products does not cover the way from memory where no second query
+// tile shares the rows.  open: the second run, for the tiles with a query that is.
+template <int R, bool SCALED>
+__global__ void __launch_bounds__(512, 2) f8_search_big_kernel(F8View V, F8Mat q, MfmaParams P, const F8State* open) {
+    using T = F8Pp<SCALED>;
     extern __shared__ __align__(16) unsigned char smem[];
-    float* thr_l = reinterpret_cast<float*>(smem + F8Pp::LDS);
+    float* thr_l = reinterpret_cast<float*>(smem + T::LDS);
     unsigned* cnt_l = reinterpret_cast<unsigned*>(thr_l + 256);
     unsigned* kept_l = cnt_l + 256;
     unsigned* flag_l = kept_l + 256;
-    F8Pp t;
+    T t;
     t.init(smem, V.X.ld / kF8Block);
     int logical = blockIdx.x;
     if ((gridDim.x & 7) == 0) logical = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     const int slice = logical / P.nqt, qt = logical % P.nqt;
     const int q0 = qt * 256;
+    if (open && !__syncthreads_or(threadIdx.x < 256 && q0 + (int)threadIdx.x < P.nq && open[q0 + threadIdx.x].ticket != 0)) return;
     const long long r_begin = (long long)slice * P.rows_per_slice;
     const long long r_end = min(r_begin + P.rows_per_slice, V.X.nrows);
     skey_t* cand = P.cand + (size_t)blockIdx.x * 256 * CAND_CAP;
@@ -949,7 +1080,7 @@ __global__ void __launch_bounds__(512, 2) f8_search_big_kernel(F8View V, F8Mat q
     if (r_begin < r_end) aim(r_begin);
 #pragma unroll 1
     for (long long row0 = r_begin; row0 < r_end; row0 += 256) {
-        F8Pp::Acc acc;
+        typename T::Acc acc;
         zero_acc(acc);
         t.run(acc);
         const long long left = r_end - row0;
@@ -1037,6 +1168,12 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
         const long long tiles = (nrows + 255) / 256;
         const auto few = [&](int tq) { return tiles * ((nq + tq - 1) / tq) <= 7ll * num_cu; };
         p->tq = nq <= 64 || few(64) ? 64 : nq <= 128 || few(128) ? 128 : 256;
+        // The scaled instruction's sums prove a list where the gap between the k-th score and the last candidate's is wide: over 1M Gaussian rows x 4096
+        // that of 16 spare ranks is seven times the error bound at k = 10 and three times at 32, where a tile of 256 queries nearly always has one that
+        // needs better sums; 32 spare ranks are five times.  (32 for all cost 1.5 times as much over 2M x 128.)  1M x 4096, 1024 queries: k = 10
+        // 4.0 ms, k = 32 4.55 (10.1 with 16), fp32 sums alone 6.65 and 6.95; where the scaled ones prove nothing (a strong channel) 10.4 and 11.5.
+        p->scaled = p->tq == 256 && k <= 32;
+        if (p->scaled && k > 16) p->kp = k + 32;
         p->nqt = (nq + p->tq - 1) / p->tq;
         const long long ns = std::max<long long>(1, std::min<long long>(num_cu / p->nqt, tiles));
         p->rows_per_slice = (tiles + ns - 1) / ns * 256;
@@ -1044,13 +1181,13 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
         p->parts = p->nslices;
         p->grid_x = p->nqt * p->nslices;
         p->threads = 512;
-        p->lds = (size_t)(p->tq == 256 ? F8Pp::LDS : p->tq == 128 ? F8Tile<4, 4, 4, 2, 3>::LDS : F8Tile<2, 4, 8, 1, 3>::LDS) + EPI_LDS_BYTES;
+        p->lds = (size_t)(p->tq == 256 ? F8Pp<false>::LDS : p->tq == 128 ? F8Tile<4, 4, 4, 2, 3>::LDS : F8Tile<2, 4, 8, 1, 3>::LDS) + EPI_LDS_BYTES;
         p->cand_bytes = (size_t)p->grid_x * 256 * CAND_CAP * sizeof(skey_t);
         // scores every slice publishes per query: enough that the kp-th largest of all of them exists and is tight (mfma.hip)
         int m = (int)((std::max<long long>(64, (long long)p->kp * 5 / 4) + p->nslices - 1) / p->nslices);
         m = std::max(1, std::min(std::min(m, 8), p->kp));
         p->gtop_m = (p->tq == 256 && p->nslices > 1 && (long long)p->nslices * m >= p->kp) ? m : 0;
-        p->share_bytes = (size_t)p->nqt * p->tq * (1 + (size_t)p->nslices * p->gtop_m) * sizeof(unsigned);
+        p->share_bytes = (size_t)p->nqt * p->tq * (1 + (size_t)p->nslices * p->gtop_m) * sizeof(unsigned) * (p->scaled ? 2 : 1);
         p->kernel = p->tq == 256 ? "f8_search_big_kernel" : "f8_search_tile_kernel";
     }
     p->partial_bytes = (size_t)nq * p->parts * p->kp * sizeof(skey_t);
@@ -1096,6 +1233,13 @@ hipError_t launch_f8_finish(const F8ScanArgs& a, const F8SearchPlan& p, hipStrea
     }
     return hipErrorInvalidValue;
 }
+hipError_t launch_f8_collect(const F8ScanArgs& a, int num_cu, hipStream_t s) {
+    const int lds = F8CollectTile::LDS + 256 * 4 + 16 + kF8Batch * 2;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_collect_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(f8_collect_kernel, dim3((unsigned)num_cu), dim3(512), lds, s, a);
+    return hipGetLastError();
+}
 hipError_t launch_f8_exact(const F8ScanArgs& a, int num_cu, hipStream_t s) {
     const int ld = a.v.X.ld;
     const size_t lds = kExactEntries * 12 + 16 + kF8Batch * 2 + kExactThreads * 4 + (size_t)(ld + ld / kF8Block + 15) / 16 * 16;
@@ -1130,15 +1274,20 @@ static hipError_t launch_tile(const F8View& v, const F8Mat& q, const F8SearchPla
     return hipGetLastError();
 }
 template <int R>
-static hipError_t launch_r(const F8View& v, const F8Mat& q, const F8SearchPlan& p, const MfmaParams& P, hipStream_t s) {
+static hipError_t launch_r(const F8View& v, const F8Mat& q, const F8SearchPlan& p, const MfmaParams& P, const F8State* open, hipStream_t s) {
     if (p.tq == 64) return launch_tile<2, 4, 8, 1, R>(v, q, p, P, s);
     if (p.tq == 128) return launch_tile<4, 4, 4, 2, R>(v, q, p, P, s);
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f8_search_big_kernel<R>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(f8_search_big_kernel<R>, dim3(p.grid_x), dim3(p.threads), p.lds, s, v, q, P);
-    return hipGetLastError();
+    const auto big = [&](auto kernel) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(kernel, dim3(p.grid_x), dim3(p.threads), p.lds, s, v, q, P, open);
+        return hipGetLastError();
+    };
+    if constexpr (R == 1)
+        if (p.scaled && !open) return big(f8_search_big_kernel<R, true>);
+    return big(f8_search_big_kernel<R, false>);
 }
-hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& p, void* share, void* cand, skey_t* partial, hipStream_t s) {
+hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& p, const F8State* open, void* share, void* cand, skey_t* partial, hipStream_t s) {
     MfmaParams P = {};
     P.nq = (int)q.n;
     P.k = p.kp;
@@ -1148,20 +1297,20 @@ hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& 
     P.partial = partial;
     P.cand = static_cast<skey_t*>(cand);
     P.thr_floor = SSMI_NEG_MAX;
-    P.gthr = static_cast<unsigned*>(share);
+    const size_t words = p.share_bytes / sizeof(unsigned);
+    P.gthr = static_cast<unsigned*>(share) + (open ? words / 2 : 0);   // (of its own for each run)
     P.gtop = p.gtop_m ? P.gthr + (size_t)p.nqt * p.tq : nullptr;
     P.gtop_m = p.gtop_m;
     P.fold_mask = P.gtop ? 0x11111111u : 0x55555555u;   // scheduled folds after row tiles 1, 16, 256, ... (1, 4, 16, ... without the bound)
     // (where first thresholds are there and two tiles follow at most, the first fold costs more than it saves: 100000 x 4096, 64 queries 201 us, 179 without)
     if (p.kp <= 64 && p.rows_per_slice <= 3 * 256) P.fold_mask &= ~1u;
-    const size_t words = p.share_bytes / sizeof(unsigned);
-    hipLaunchKernelGGL(f8_zero_kernel, dim3((unsigned)std::min<size_t>((words + 255) / 256, 4096)), dim3(256), 0, s, P.gthr, words);
+    if (!open) hipLaunchKernelGGL(f8_zero_kernel, dim3((unsigned)std::min<size_t>((words + 255) / 256, 4096)), dim3(256), 0, s, P.gthr, words);
     switch (p.r) {
-        case 1: return launch_r<1>(v, q, p, P, s);
-        case 2: return launch_r<2>(v, q, p, P, s);
-        case 4: return launch_r<4>(v, q, p, P, s);
-        case 8: return launch_r<8>(v, q, p, P, s);
-        case 16: return launch_r<16>(v, q, p, P, s);
+        case 1: return launch_r<1>(v, q, p, P, open, s);
+        case 2: return launch_r<2>(v, q, p, P, open, s);
+        case 4: return launch_r<4>(v, q, p, P, open, s);
+        case 8: return launch_r<8>(v, q, p, P, open, s);
+        case 16: return launch_r<16>(v, q, p, P, open, s);
     }
     return hipErrorInvalidValue;
 }

@@ -7,9 +7,10 @@
 // (exact from 2^-133 to the end of fp32; scale byte 255 gives NaN), and at 4 cycles a pair it hides under v_mfma_f32_*_bf16.
 // Products of such operands are exact and the sums are fp32's: measured, an instruction is off by less than 2^-21.5 of the
 // magnitudes it adds, 2^-22 of an accumulator that is large beside them.
-// v_mfma_scale_f32_*_f8f6f4, which takes codes and scale bytes as they are at twice the rate (3.9 PFLOP/s on registers, 1.75), is not
-// used: it aligns the products of eight neighbouring codes to the largest of them and drops what lies more than 13 bits below
-// (measured; v_mfma_f32_*_fp8_fp8 does the same), so that a strong channel or two large products that cancel take the rest with them.
+// v_mfma_scale_f32_*_f8f6f4, which takes codes and scale bytes as they are at twice the rate (3.9 PFLOP/s on registers, 1.75), aligns the products
+// of eight neighbouring codes to the largest of them and drops what lies more than 13 bits below (measured; v_mfma_f32_*_fp8_fp8 does the
+// same), so that a strong channel or two large products that cancel take the rest with them.  Only a search that checks what that
+// may have cost it uses it (f8_pp.h, f8_search.hip).
 #pragma once
 #include "f8.h"
 #include "mfma_common.h"
@@ -38,6 +39,11 @@ __device__ __forceinline__ f32x4_t mfma_f8(const i32x4_t& a, const i32x4_t& b, c
 }
 __device__ __forceinline__ f32x16_t mfma_f8_32(const i32x4_t& a, const i32x4_t& b, const f32x16_t& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+// ... and with the scaled instruction: 64 codes of K
+template <int J>
+__device__ __forceinline__ f32x16_t mfma_f8_scaled(const i32x8_t& a, const i32x8_t& b, const f32x16_t& c, int sa, int sb) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, J, sa, J, sb);
 }
 __device__ __forceinline__ i32x8_t join8(const i32x4_t& lo, const i32x4_t& hi) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -102,6 +108,11 @@ struct F8Tile {
     // sources of a tile; starts its pipeline (the first S - 1 slabs).  No wave may still read the ring: true at the start and
     // whenever run() has returned
     __device__ __forceinline__ void aim(const F8Src& x, const F8Src& q) {
+        aim(x, q, [](int r) __attribute__((always_inline)) { return r; });
+    }
+    // ... query r of the tile is row qrow(r) of q
+    template <typename F>
+    __device__ __forceinline__ void aim(const F8Src& x, const F8Src& q, F qrow) {
 #pragma unroll
         for (int j = 0; j < PX; ++j) {
             const int r = (wave * PX + j) * 8 + (lane >> 3);
@@ -110,14 +121,14 @@ struct F8Tile {
 #pragma unroll
         for (int j = 0; j < PQ; ++j) {
             const int r = (wave * PQ + j) * 8 + (lane >> 3);
-            qo[j] = (unsigned)min(r, q.last) * q.stride + (((lane & 7) ^ ((r >> 1) & 7)) * 16);
+            qo[j] = (unsigned)qrow(min(r, q.last)) * q.stride + (((lane & 7) ^ ((r >> 1) & 7)) * 16);
         }
         xc = x.codes;
         qc = q.codes;
 #pragma unroll
         for (int j = 0; j < PW; ++j) {
             const int r = word_piece(j) * 64 + lane;
-            sc[j] = r < XR ? x.scales + (unsigned)min(r, x.last) * x.sstride : q.scales + (unsigned)min(r - XR, min(q.last, QR - 1)) * q.sstride;
+            sc[j] = r < XR ? x.scales + (unsigned)min(r, x.last) * x.sstride : q.scales + (unsigned)qrow(max(0, min(r - XR, min(q.last, QR - 1)))) * q.sstride;
         }
 #pragma unroll
         for (int d = 0; d < S - 1; ++d)

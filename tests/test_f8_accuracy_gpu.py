@@ -204,3 +204,25 @@ def test_norm_is_the_64_bit_norm_rounded_once(ssa, name, unit, t):
     got = plain.values(rows.codes.view(torch.uint8).cpu().numpy(), rows.scales.cpu().numpy(), rows.d)
     assert ((got == lo) | (got == hi)).all()
     assert np.mean(lo != hi) < 1e-6   # (the borders leave the rest nothing to hide in)
+
+
+@pytest.mark.parametrize("k", [1, 10, 32, 33])
+@pytest.mark.parametrize("d", [64, 300, 1024])
+@pytest.mark.parametrize("kind", ["generic", "strong", "copies", "all"])
+def test_large_batches_whose_lists_are_proven_by_different_sums(ssa, kind, d, k):
+    """Enough rows and queries for the largest tiles: queries that their first sums answer, queries that need better ones, queries that
+    need all rows in 64 bits, in tiles of their own and together."""
+    n, nq = 140000, 700
+    g = torch.Generator(device="cuda").manual_seed(SALT + d + k)
+    unit = torch.nn.functional.normalize
+    x, q = unit(torch.randn(n, d, generator=g, device="cuda")), unit(torch.randn(nq, d, generator=g, device="cuda"))
+    if kind in ("strong", "all"):
+        some, few = (slice(0, n), slice(0, nq)) if kind == "strong" else (slice(90000, n), slice(400, 500))
+        x[some] *= 0.02
+        x[some, 7] = 1
+        q[few] *= 0.02
+        q[few, 7] = 1
+    if kind in ("copies", "all"):
+        x[1000:1300] = x[1000]
+        q[300:310] = x[1000]
+    check_search(ssa, ssa.quantize_f8(x), ssa.quantize_f8(q), k)

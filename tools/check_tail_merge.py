@@ -22,8 +22,8 @@ import sys
 
 # kernels whose last workgroup reads so many pointers behind the merge
 POINTER_LOADS = {"f8_scan_kernel": 8}
-# kernels that count workgroups with release and acquire fences and hand over nothing without
-FENCED = ("f8_exact_kernel",)
+# kernels whose counters are no tickets of this protocol: one goes by release and acquire fences, one fills lists for the next launch
+FENCED = ("f8_exact_kernel", "f8_collect_kernel")
 
 
 def kernels(path):
