@@ -355,7 +355,11 @@ __global__ void __launch_bounds__(1024) f8_finish_kernel(F8ScanArgs A, int P) {
 // their numbers: from the front of list those that are to see all rows (n[0] of them), from the back the others (n[1]).  All threads
 __device__ __forceinline__ void open_queries(const F8ScanArgs& A, unsigned short* list, unsigned* n) {
     const int lane = lane_id(), nq = (int)A.q.n;
-    if (threadIdx.x < 64) {
+    bool any = false;
+    for (int q = threadIdx.x; q < nq; q += blockDim.x) any |= __hip_atomic_load(&A.state[q].ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
+    if (!__syncthreads_or(any)) {   // (as a rule)
+        if (threadIdx.x == 0) n[0] = n[1] = 0;
+    } else if (threadIdx.x < 64) {
         int all = 0, few = 0;
         for (int q0 = 0; q0 < nq; q0 += 64) {
             const F8State* st = A.state + min(q0 + lane, nq - 1);
@@ -615,14 +619,18 @@ __global__ void __launch_bounds__(256) f8_lengths_kernel(F8Mat m, int ld, float*
     }
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) { most = fmaxf(most, __shfl_xor(most, d)); most8 = fmaxf(most8, __shfl_xor(most8, d)); }
-    if (lane == 0) {
-        if (most > 0.f) atomicMax(longest, __float_as_uint(most));
-        if (most8 > 0.f) atomicMax(longest + 1, __float_as_uint(most8));
+    // (one atomic a workgroup at most: one a wave took longer than the rows)
+    __shared__ float part[4][2];
+    if (lane == 0) { part[wave][0] = most; part[wave][1] = most8; }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const float v = fmaxf(fmaxf(part[0][threadIdx.x], part[1][threadIdx.x]), fmaxf(part[2][threadIdx.x], part[3][threadIdx.x]));
+        if (v > __uint_as_float(__hip_atomic_load(longest + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))) atomicMax(longest + threadIdx.x, __float_as_uint(v));
     }
 }
 hipError_t launch_f8_lengths(const F8Mat& m, int ld, float* lengths, unsigned* longest, int num_cu, hipStream_t s) {
     if (m.n <= 0) return hipSuccess;
-    const long long blocks = (m.n + 3) / 4, most = (long long)num_cu * 8;
+    const long long blocks = (m.n + 3) / 4, most = (long long)num_cu * 4;
     hipLaunchKernelGGL(f8_lengths_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, m, ld, lengths, longest);
     return hipGetLastError();
 }
