@@ -31,7 +31,7 @@ for kernels in out.values():
         if v.get("GRBM_GUI_ACTIVE") and "SQ_VALU_MFMA_BUSY_CYCLES" in v:
             # (GRBM counts per XCD, SQ per SIMD: 8 XCDs, 1024 SIMDs)
             v["matrix_pipe_busy"] = round(v["SQ_VALU_MFMA_BUSY_CYCLES"] / (v["GRBM_GUI_ACTIVE"] / 8 * 1024), 3)
-            if "us" in v:
+            if v.get("us", 0) > 100:   # (shorter ones are not alone in the counted time)
                 v["clock_GHz"] = round(v["GRBM_GUI_ACTIVE"] / 8 / v["us"] / 1e3, 2)
         if "FETCH_SIZE" in v:
             v["read_GB"] = round(v["FETCH_SIZE"] * 2048 / 1e9, 3)   # (KiB; half of a wide coalesced read is counted)

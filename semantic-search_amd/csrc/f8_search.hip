@@ -333,8 +333,8 @@ __device__ __forceinline__ void stage_query(const F8ScanArgs& A, long long b, un
     }
 }
 
-// what follows the first pass where it does not carry it: one workgroup per query.  A chain of memory round trips and sorts: 16 us for
-// 8 queries of 256 lists, 42 us for 1024 of 40
+// what follows the first pass where it does not carry it: one workgroup per query.  A chain of memory round trips and sorts: 17 us for
+// 64 queries of 40 lists, 52 us for 1024 of 64
 template <int R>
 __global__ void __launch_bounds__(1024) f8_finish_kernel(F8ScanArgs A, int P) {
     extern __shared__ __align__(16) unsigned char smem[];
@@ -1153,10 +1153,9 @@ bool plan_f8_search(int ld, long long nrows, int nq, int k, int num_cu, F8Search
         p->nb = nblk == 1 || nblk == 2 || nblk == 4 ? nblk : nblk % 8 == 0 ? 8 : 0;
         const int run_rows = p->nb ? 64 / p->nb : 8, stages = (nblk + 7) / 8;
         const long long runs = (nrows + run_rows - 1) / run_rows;
-        // One workgroup per CU.  Whole stages keep six waves' worth of loads ahead of memory and eight only share the buffers with
-        // more (1M x 4096, one query: 611 us with six, 641 us with eight); where a wave has a handful of runs, or short
-        // stages, eight (10k x 4096: 30.0 us, with six 32.9; 2M x 768: 285 and 308).
-        const int waves = p->nb == 8 && runs >= 24ll * num_cu ? 6 : 8;
+        // One workgroup per CU, of eight waves: six hold as many rows in flight but convert fewer of them meanwhile (one query, us with 4, 6 and 8 waves:
+        // 10000 x 4096 43.0, 37.6, 34.4; 1M x 1024 254, 194, 177; 2M x 768 462, 340, 285; 1M x 4096 758, 623, 616; only 200000 x 8192 330, 283, 294).
+        const int waves = 8;
         p->threads = waves * 64;
         // The waves look at the candidate buffers at most p->every turns of three stages apart: no query may gain more rows
         // meanwhile than its buffer holds beside the 63 candidates that a look may leave
@@ -1310,7 +1309,8 @@ hipError_t launch_f8_tiles(const F8View& v, const F8Mat& q, const F8SearchPlan& 
     P.gtop = p.gtop_m ? P.gthr + (size_t)p.nqt * p.tq : nullptr;
     P.gtop_m = p.gtop_m;
     P.fold_mask = P.gtop ? 0x11111111u : 0x55555555u;   // scheduled folds after row tiles 1, 16, 256, ... (1, 4, 16, ... without the bound)
-    // (where first thresholds are there and two tiles follow at most, the first fold costs more than it saves: 100000 x 4096, 64 queries 201 us, 179 without)
+    // (where first thresholds are there and two tiles follow at most, the first fold costs more than it saves: 100000 x 4096, 64 queries 210 us, 188 without, 100000 x 1024 138 and 111; where four
+    // follow it pays: 100000 x 4096, 128 queries 256 us, 263 without)
     if (p.kp <= 64 && p.rows_per_slice <= 3 * 256) P.fold_mask &= ~1u;
     if (!open) hipLaunchKernelGGL(f8_zero_kernel, dim3((unsigned)std::min<size_t>((words + 255) / 256, 4096)), dim3(256), 0, s, P.gthr, words);
     switch (p.r) {
