@@ -72,7 +72,8 @@ hipError_t launch_f8_lengths(const F8Mat& m, int ld, float* lengths, unsigned* l
 
 // What the second pass of a search leaves for the third.  ticket 0: the query is answered; else it counts the workgroups that are done with it,
 // from 1, and pos their entries.  No row with a score below edge is among the k best, nor one that is not on the list and shorter than `from`,
-// nor one whose fp32 sum s and length x have s + slope x < least.  found: how many rows have not, more than kF8Collect: unknown
+// nor one whose fp32 sum s and length x have s + slope x < least (slope < 0: that is not known).  found: how many rows have not, more than kF8Collect:
+// they are not listed
 struct F8State { double edge; float from, least, slope; unsigned ticket, pos, found; };
 struct F8Entry { double score; long long id; };
 

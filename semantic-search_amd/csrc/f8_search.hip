@@ -196,7 +196,7 @@ __device__ __forceinline__ void finish_query(const F8ScanArgs& A, long long qi, 
         const bool sums = valid >= k && p.last != 0 && q < 1e37 && x < 1e37 && q * x < 1e37;   // no sum leaves fp32
         // (rounded outwards, and the sum that is compared with it is off by 2^-24 of itself)
         const float least = (float)(p.kth - fabs(p.kth) * 0x1p-22 - 0x1p-118 * (q + x) - 0x1p-125), slope = (float)(f8_relative(V.X.ld / kF8Block) * q * (1 + 0x1p-20));
-        A.state[qi] = F8State{valid >= k ? p.kth : -__builtin_inf(), from, sums ? least : 0.f, sums ? slope : 0.f, proven ? 0u : 1u, 0u, sums && A.open ? 0u : kF8Collect + 1u};
+        A.state[qi] = F8State{valid >= k ? p.kth : -__builtin_inf(), from, least, sums && A.open ? slope : -1.f, proven ? 0u : 1u, 0u, sums && A.open ? 0u : kF8Collect + 1u};
         L.proof->last = proven || A.sums == kF8Scaled || !A.open ? 0 : 1;
     }
     __syncthreads();
@@ -352,8 +352,11 @@ __global__ void __launch_bounds__(1024) f8_finish_kernel(F8ScanArgs A, int P) {
 }
 
 // ---- third pass: the queries that are not proven.  A workgroup per CU ----
-// their numbers: from the front of list those that are to see all rows (n[0] of them), from the back the others (n[1]).  All threads
-__device__ __forceinline__ void open_queries(const F8ScanArgs& A, unsigned short* list, unsigned* n) {
+// their numbers: from the front of list those that are to see all rows by whole(state) (n[0] of them), from the back the others (n[1]).  Every
+// workgroup of a launch makes the list for itself and takes its share of it, so whole() goes by what no workgroup of that launch writes, as
+// does the ticket's being zero.  All threads
+template <typename F>
+__device__ __forceinline__ void open_queries(const F8ScanArgs& A, unsigned short* list, unsigned* n, F whole_of) {
     const int lane = lane_id(), nq = (int)A.q.n;
     bool any = false;
     for (int q = threadIdx.x; q < nq; q += blockDim.x) any |= __hip_atomic_load(&A.state[q].ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
@@ -364,7 +367,7 @@ __device__ __forceinline__ void open_queries(const F8ScanArgs& A, unsigned short
         for (int q0 = 0; q0 < nq; q0 += 64) {
             const F8State* st = A.state + min(q0 + lane, nq - 1);
             const bool is = q0 + lane < nq && __hip_atomic_load(&st->ticket, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
-            const bool whole = is && st->found > (unsigned)kF8Collect;
+            const bool whole = is && whole_of(*st);
             const unsigned long long ma = __builtin_amdgcn_ballot_w64(whole), mf = __builtin_amdgcn_ballot_w64(is && !whole), below = (1ull << lane) - 1;
             if (whole) list[all + __builtin_popcountll(ma & below)] = (unsigned short)(q0 + lane);
             else if (is) list[kF8Batch - 1 - few - __builtin_popcountll(mf & below)] = (unsigned short)(q0 + lane);
@@ -377,8 +380,9 @@ __device__ __forceinline__ void open_queries(const F8ScanArgs& A, unsigned short
 }
 
 // Scores as finish_query's.  A query whose rows in question are known has a workgroup score those.  Of the others, W workgroups share one (all of the
-// grid if it is alone); each takes a range of the rows, picks those that are long enough and keeps what may be among the k best in LDS, sorted down to k whenever the buffer fills; the last to finish joins their lists.  1M x 4096 with every row long enough: 1.4 ms
-// for one query, 0.8 ms for each of many, by the vector units (four instructions a product).  With nothing to do the launch costs 3 us.
+// grid if it is alone); each takes a range of the rows, picks those that are long enough and keeps what may be among the k best in LDS, sorted
+// down to k whenever the buffer fills; the last to finish joins their lists.  1M x 4096 with every row long enough: 1.4 ms for one query, 0.8
+// ms for each of many, by the vector units (four instructions a product).  With nothing to do the launch costs 3 us.
 static constexpr int kExactThreads = 1024, kExactEntries = 2048, kExactRound = 256;   // entries of a buffer, and how many a round may add
 struct F8Exact {
     double* score;
@@ -439,7 +443,7 @@ __global__ void __launch_bounds__(kExactThreads) f8_exact_kernel(F8ScanArgs A) {
     unsigned* sel = reinterpret_cast<unsigned*>(open + kF8Batch);            // [blockDim.x] rows of a round
     unsigned char* qs = reinterpret_cast<unsigned char*>(sel + blockDim.x);
     unsigned char* qsc = qs + ld;
-    open_queries(A, open, X.count + 1);
+    open_queries(A, open, X.count + 1, [](const F8State& st) __attribute__((always_inline)) { return st.found > (unsigned)kF8Collect; });
     const int nall = __builtin_amdgcn_readfirstlane((int)X.count[1]), nfew = __builtin_amdgcn_readfirstlane((int)X.count[2]);
     if (nall + nfew == 0) return;
     const int W = nall ? max(1, (int)gridDim.x / nall) : 1;
@@ -545,7 +549,7 @@ __global__ void __launch_bounds__(512) f8_collect_kernel(F8ScanArgs A) {
     unsigned short* open = reinterpret_cast<unsigned short*>(count + 4);      // [kF8Batch]
     const F8View& V = A.v;
     const int ld = V.X.ld;
-    open_queries(A, open, count);
+    open_queries(A, open, count, [](const F8State& st) __attribute__((always_inline)) { return !(st.slope >= 0.f); });   // (not by found, which grows)
     const int nopen = __builtin_amdgcn_readfirstlane((int)count[1]);
     if (nopen == 0) return;
     T t;

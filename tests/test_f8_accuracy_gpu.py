@@ -208,7 +208,7 @@ def test_norm_is_the_64_bit_norm_rounded_once(ssa, name, unit, t):
 
 @pytest.mark.parametrize("k", [1, 10, 32, 33])
 @pytest.mark.parametrize("d", [64, 300, 1024])
-@pytest.mark.parametrize("kind", ["generic", "strong", "copies", "all"])
+@pytest.mark.parametrize("kind", ["generic", "strong", "copies", "all", "half"])
 def test_large_batches_whose_lists_are_proven_by_different_sums(ssa, kind, d, k):
     """Enough rows and queries for the largest tiles: queries that their first sums answer, queries that need better ones, queries that
     need all rows in 64 bits, in tiles of their own and together."""
@@ -225,4 +225,32 @@ def test_large_batches_whose_lists_are_proven_by_different_sums(ssa, kind, d, k)
     if kind in ("copies", "all"):
         x[1000:1300] = x[1000]
         q[300:310] = x[1000]
+    if kind == "half":   # more copies than are listed, and long rows that leave the other queries rows in question
+        x[:5000] = x[0]
+        q[:350] = x[0]
+        x[70000] *= 1e5
     check_search(ssa, ssa.quantize_f8(x), ssa.quantize_f8(q), k)
+
+
+def test_searches_with_open_queries_on_two_streams(ssa):
+    """Both keep their open queries in the handle's workspaces: one waits for the other."""
+    g = torch.Generator(device="cuda").manual_seed(SALT + 9)
+    x, q = (torch.nn.functional.normalize(torch.randn(c, 300, generator=g, device="cuda")) for c in (30000, 400))
+    x[100:200] = x[100]
+    q[::3] = x[100]
+    x[7] *= 1e5
+    rows, queries = ssa.quantize_f8(x), ssa.quantize_f8(q)
+    index = ssa.IndexFlatIP(300, storage="f8")
+    index.add(rows)
+    _, ids = exact_search(rows, queries, 20)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(12):
+        lo, hi = [(0, 400), (0, 1), (5, 9), (100, 130)][i % 4]
+        part = queries[lo:hi]
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((lo, hi, part, index.search(part, 20)[1]))
+    torch.cuda.synchronize()
+    for lo, hi, _, I in got:
+        assert torch.equal(I, ids[lo:hi])
