@@ -641,7 +641,7 @@ hipError_t launch_f8_lengths(const F8Mat& m, int ld, float* lengths, unsigned* l
 
 // ---- streaming scan: up to BT <= 8 queries ----
 // Bound by reading the rows once; what reads fastest decides the layout.  A plain read of 1M x 4096 codes ran at 5.9 TB/s with
-// 16 rows x 64 bytes per load instruction (the operand layout of the 16x16x128 instruction as it is) and at 6.7-7.0 TB/s with 8
+// 16 rows x 64 bytes per load instruction (a matrix instruction's sixteen rows as they are) and at 6.7-7.0 TB/s with 8
 // rows x 128 bytes, non-temporal loads and 4-8 waves per CU.  So one load is one whole block of eight rows, 16 codes a lane,
 // and feeds two instructions of K = 32 (f8_tile.h): the sixteen operand rows
 // are the 8 rows x {even, odd 16-byte chunks}, the sixteen columns 8 queries x {even, odd chunks}, and a score is the

@@ -236,7 +236,8 @@ def rms_norm_f8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual
 
 
 def matmul_f8(a: F8Rows, b: F8Rows, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """(a.n, b.n): inner products of the rows of a (activations) with the rows of b (weights, or a table of embeddings)."""
+    """(a.n, b.n): inner products of the rows of a (activations) with the rows of b (weights, or a table of embeddings), exact products
+    summed in float32 and rounded once to the output's type."""
     if not isinstance(a, F8Rows) or not isinstance(b, F8Rows):
         raise TypeError("matmul_f8: expected two F8Rows")
     if a.d != b.d:

@@ -13,7 +13,7 @@ BUILD = os.path.join(ROOT, "semantic-search_amd", "csrc", "build")
 OBJDUMP = "/opt/rocm/lib/llvm/bin/llvm-objdump"
 
 
-def checker():
+def tail_check():
     spec = importlib.util.spec_from_file_location("check_tail_merge", os.path.join(ROOT, "tools", "check_tail_merge.py"))
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
@@ -39,16 +39,16 @@ def test_built_kernels_publish_drain_and_read_past_their_cache(obj, min_kernels,
             listing.append("\t" + line.split("//")[0].strip())
     out = tmp_path / "k.s"
     out.write_text("\n".join(listing + [".Lfunc_end:"]))
-    assert checker().main(str(out)) == 0, capsys.readouterr().out[-2000:]
+    assert tail_check().main(str(out)) == 0, capsys.readouterr().out[-2000:]
     report = capsys.readouterr().out
     assert int(report.strip().split("\n")[-1].split()[0]) >= min_kernels, report[-500:]
 
 
-def test_the_checker_reports_pointers_that_are_lists(tmp_path, capsys):
+def test_lists_among_the_pointers_are_reported(tmp_path, capsys):
     """Of the scan of 8-bit rows it lets eight plain loads pass, behind the lists' and nowhere else."""
     head = "_ZN4ssmi14f8_scan_kernelEv:\n\tglobal_store_dwordx2 v[0:1], v[2:3], off sc1\n\ts_waitcnt vmcnt(0)\n\tglobal_atomic_add v1, v1, v4, s[0:1] sc0\n"
     coherent, plain = "\tglobal_load_dwordx2 v[0:1], v[2:3], off sc1\n", "\tglobal_load_dwordx2 v[0:1], v2, s[2:3]\n"
     for body, status in ((coherent * 3 + plain * 8, 0), (coherent * 2 + plain * 9, 1), (plain + coherent * 3 + plain * 8, 1), (coherent * 3 + plain * 7 + coherent, 1)):
         f = tmp_path / "f.s"
         f.write_text(head + body + ".Lfunc_end0:\n")
-        assert checker().main(str(f)) == status
+        assert tail_check().main(str(f)) == status
